@@ -1,0 +1,334 @@
+// What fills the cache of 4 bits an element (four_bit.h) and what reads it back as values.
+//
+// Filling it: a row of the fused q/k/v projection becomes query heads (RMS norm of the head times a gain, rotation; rounded once, to
+// the engine's type) and cached keys and values.  A key is normed and rotated in 64 bits and stays there up to its codes: which
+// of two neighbouring codes an element gets is decided by a comparison, and one that lies next to the border between
+// them falls on its own side whatever order the squares were added in.  (The 64-bit instructions are a third of a key's, and the
+// launch waits for its rows.)  Values are only scaled by a power of two, which float does exactly.
+//
+// A lane has eight neighbouring elements, a head dim / 8 lanes (rounded up to a power of two), a wave as many rows of one
+// head as fit: four rows of 128.  So a wave's keys of a block and its values of eight elements are neighbouring bytes of the cache
+// where its rows are neighbouring tokens, and the four lanes of a block find its largest element by two exchanges.  The
+// partners of a rotation in halves are loaded a second time (from the first-level cache) instead of being exchanged.
+#include "common.h"
+#include "four_bit.h"
+#include "leone_hip.h"
+
+#include <math.h>
+
+namespace leone {
+
+constexpr int kFillThreads = 256;
+
+struct FillShape {
+    int rows, q_heads, kv_heads, dim, page_tokens, max_blocks, entries;
+    long row_width;              // elements from row to row
+    int planes;
+    long plane;
+    float eps;
+    const float* cos_table;      // [table_positions, rotary_half], null: no rotation
+    const float* sin_table;
+    int table_positions, rotary_half, pairing;
+};
+
+// Eight neighbouring elements of a row, the planes of a product cut along K added up in order.
+template <typename TIn, typename Acc>
+__device__ inline void load_eight(const TIn* __restrict__ from, int planes, long plane, Acc out[8]) {
+    float part[8];
+    constexpr int code = sizeof(TIn) == 4 ? kF32 : kBF16;
+    load_any8(AnyVec{from, code}, 0, part);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = static_cast<Acc>(part[i]);
+    for (int s = 1; s < planes; ++s) {
+        load_any8(AnyVec{from, code}, s * plane, part);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out[i] += static_cast<Acc>(part[i]);
+    }
+}
+
+__device__ inline float root(float v) { return sqrtf(v); }
+__device__ inline double root(double v) { return sqrt(v); }
+
+// Eight elements of a query or key head: normed and rotated.  `at` is the lane's first element; lanes behind the head (at >= dim)
+// take part in the sum with nothing.
+template <int kSpan, typename TIn, typename Acc>
+__device__ inline void make_eight(const TIn* __restrict__ head, int at, const FillShape& s, const AnyVec& gain, int pos, Acc x[8]) {
+    const bool in_head = at < s.dim;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0;
+    if (in_head) load_eight<TIn, Acc>(head + at, s.planes, s.plane, x);
+    // the partners, where they are not among the lane's own
+    const int half = s.rotary_half;
+    const bool turned = s.cos_table != nullptr && at < 2 * half;
+    const bool apart = turned && s.pairing == 0;
+    Acc other[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) other[i] = 0;
+    auto partner = [&](int d) { return d < half ? d + half : d - half; };
+    if (apart && in_head) {
+        if (half % 8 == 0) {
+            load_eight<TIn, Acc>(head + partner(at), s.planes, s.plane, other);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (at + i < 2 * half)
+                    for (int p = 0; p < s.planes; ++p) {
+                        const TIn v = head[p * s.plane + partner(at + i)];
+                        other[i] += static_cast<Acc>(to_float(v));
+                    }
+        }
+    }
+    if (gain.ptr) {
+        Acc squares = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) squares += x[i] * x[i];
+        squares = join_span<kSpan>(squares, [](Acc a, Acc b) { return a + b; });
+        const Acc inv = Acc(1) / root(squares / static_cast<Acc>(s.dim) + static_cast<Acc>(s.eps));
+        if (in_head) {
+            float g[8];
+            load_any8(gain, at, g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * static_cast<Acc>(g[i]) * inv;
+            if (apart) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (at + i < 2 * half) other[i] = other[i] * static_cast<Acc>(load_any(gain, partner(at + i))) * inv;
+            }
+        }
+    }
+    if (!turned) return;
+    const long angles = static_cast<long>(pos < s.table_positions ? pos : s.table_positions - 1) * half;   // (the host checks the bound)
+    if (s.pairing != 0) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            if (at + i >= 2 * half) continue;
+            const Acc c = s.cos_table[angles + (at + i) / 2], n = s.sin_table[angles + (at + i) / 2];
+            const Acc a = x[i], b = x[i + 1];
+            x[i] = a * c - b * n;
+            x[i + 1] = a * n + b * c;
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int d = at + i;
+        if (d >= 2 * half) continue;
+        const bool first = d < half;
+        const Acc c = s.cos_table[angles + (first ? d : d - half)], n = s.sin_table[angles + (first ? d : d - half)];
+        x[i] = first ? x[i] * c - other[i] * n : other[i] * n + x[i] * c;
+    }
+}
+
+// The power of a block of 32 (four neighbouring lanes) and the lane's eight codes.
+__device__ inline unsigned long long magnitude(double v) { return __builtin_bit_cast(unsigned long long, v) & 0x7fffffffffffffffull; }
+__device__ inline unsigned magnitude(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }
+__device__ inline int block_power(unsigned long long top) {
+    const int exponent = static_cast<int>(top >> 52);
+    if (exponent == 0x7ff) return kNanPower;
+    const int power = exponent - 1023 - ((top & 0xfffffffffffffull) > 0xc000000000000ull ? 1 : 2);       // above 1.75 times a power of two?
+    return min(max(power, -126), 127) + 127;
+}
+__device__ inline int block_power(unsigned top) {
+    const int exponent = static_cast<int>(top >> 23);
+    if (exponent == 0xff) return kNanPower;
+    const int power = exponent - 127 - ((top & 0x7fffffu) > 0x600000u ? 1 : 2);
+    return max(power, -126) + 127;
+}
+// x / 2^(power - 127) as a float that rounds to the same code: of a 64-bit number the float towards zero, its last bit set where
+// something was cut off.
+__device__ inline float in_units(double x, int power) {
+    const double y = x * __builtin_bit_cast(double, static_cast<unsigned long long>(1023 + 127 - power) << 52);
+    const float f = static_cast<float>(y);
+    const double back = f;
+    unsigned bits = __builtin_bit_cast(unsigned, f);
+    if (back != y) bits = (fabs(back) > fabs(y) ? bits - 1 : bits) | 1u;
+    return __builtin_bit_cast(float, bits);
+}
+__device__ inline float in_units(float x, int power) { return ldexpf(x, 127 - power); }
+
+template <typename Acc>
+__device__ inline unsigned eight_codes(const Acc x[8], int& power) {
+    decltype(magnitude(Acc())) top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, magnitude(x[i]));
+    top = join_span<4>(top, [](auto a, auto b) { return a > b ? a : b; });
+    power = block_power(top);
+    const int by = power == kNanPower ? 127 : power;
+    unsigned codes = 0;
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, in_units(x[0], by), in_units(x[1], by), 1.0f, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, in_units(x[2], by), in_units(x[3], by), 1.0f, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, in_units(x[4], by), in_units(x[5], by), 1.0f, 2);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, in_units(x[6], by), in_units(x[7], by), 1.0f, 3);
+    return codes;
+}
+
+template <int kSpan, typename TIn, typename T>
+__global__ void __launch_bounds__(kFillThreads)
+four_bit_fill_kernel(const TIn* __restrict__ qkv, T* __restrict__ q_out, FourBitPools pools, AnyVec q_gain, AnyVec k_gain,
+                     const int* __restrict__ positions, const int* __restrict__ row_entry, const int* __restrict__ block_table, FillShape s) {
+    constexpr int kRows = kWave / kSpan;                          // rows of one head a wave takes
+    const int lane = threadIdx.x % kWave;
+    const int heads = s.q_heads + 2 * s.kv_heads;
+    const long item = static_cast<long>(blockIdx.x) * (kFillThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int row_run = static_cast<int>(item / heads), head = static_cast<int>(item - static_cast<long>(row_run) * heads);
+    if (row_run * kRows >= s.rows) return;
+    const int row = row_run * kRows + lane / kSpan;
+    const int at = lane % kSpan * 8;
+    const bool exists = row < s.rows;
+    const int from_row = exists ? row : s.rows - 1;               // (every lane takes part in the exchanges)
+    const int pos = positions[from_row];
+    const TIn* from = qkv + static_cast<long>(from_row) * s.row_width + static_cast<long>(head) * s.dim;
+    if (head < s.q_heads) {
+        float x[8];
+        make_eight<kSpan, TIn, float>(from, at, s, q_gain, pos, x);
+        if (!exists || at >= s.dim) return;
+        T* to = q_out + (static_cast<long>(row) * s.q_heads + head) * s.dim + at;
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(to) = float4{x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<float4*>(to + 4) = float4{x[4], x[5], x[6], x[7]};
+        } else {
+            unsigned w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = bf16_bits_from_float(x[2 * i]) | static_cast<unsigned>(bf16_bits_from_float(x[2 * i + 1])) << 16;
+            *reinterpret_cast<uint4*>(to) = uint4{w[0], w[1], w[2], w[3]};
+        }
+        return;
+    }
+    const bool is_key = head < s.q_heads + s.kv_heads;
+    const int kvh = head - s.q_heads - (is_key ? 0 : s.kv_heads);
+    int power;
+    unsigned codes;
+    if (is_key) {
+        double x[8];
+        make_eight<kSpan, TIn, double>(from, at, s, k_gain, pos, x);
+        codes = eight_codes(x, power);
+    } else if (s.planes == 1) {
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (at < s.dim) load_eight<TIn, float>(from + at, 1, 0, x);
+        codes = eight_codes(x, power);
+    } else {
+        double x[8] = {0., 0., 0., 0., 0., 0., 0., 0.};
+        if (at < s.dim) load_eight<TIn, double>(from + at, s.planes, s.plane, x);
+        codes = eight_codes(x, power);
+    }
+    if (!exists || at >= s.dim || pos < 0) return;
+    const int entry = row_entry[row];
+    if (entry < 0 || entry >= s.entries) return;
+    const int block = pos / s.page_tokens, token = pos - block * s.page_tokens;
+    const int page = mapped_page(block_table + static_cast<long>(entry) * s.max_blocks, block, s.max_blocks, pools.pages);
+    if (page < 0) return;                                         // the host reserves the pages before the launch
+    const long place = static_cast<long>(page) * s.kv_heads + kvh;
+    const long code_base = place * four_bit_codes(s.page_tokens, s.dim), power_base = place * four_bit_powers(s.page_tokens, s.dim);
+    if (is_key) {
+        *reinterpret_cast<unsigned*>(pools.k_codes + code_base + four_bit_key(token, at / kBlock, s.page_tokens) + at % kBlock / 2) = codes;
+        if (at % kBlock == 0) pools.k_powers[power_base + four_bit_key_power(token, at / kBlock, s.dim)] = static_cast<uint8_t>(power);
+    } else {
+        *reinterpret_cast<unsigned*>(pools.v_codes + code_base + four_bit_value(token, at / 8, s.dim)) = codes;
+        if (at % kBlock == 0) pools.v_powers[power_base + four_bit_value_power(token, at / kBlock, s.dim)] = static_cast<uint8_t>(power);
+    }
+}
+
+// Reading rows back: a thread has eight elements of a key or a value.  A number of two bits times a power of two is a bfloat16
+// as it is.  Rows without a page give NaN.
+__global__ void __launch_bounds__(kFillThreads)
+four_bit_rows_kernel(FourBitPools pools, const int* __restrict__ positions, const int* __restrict__ row_entry, const int* __restrict__ block_table,
+                     int max_blocks, int entries, bf16_t* __restrict__ k_out, bf16_t* __restrict__ v_out, long items, int kv_heads, int dim,
+                     int page_tokens) {
+    const long item = static_cast<long>(blockIdx.x) * kFillThreads + threadIdx.x;
+    if (item >= items) return;
+    const int eights = dim / 8;
+    const long head_row = item / eights;
+    const int eight = static_cast<int>(item - head_row * eights);
+    const int row = static_cast<int>(head_row / kv_heads), kvh = static_cast<int>(head_row - static_cast<long>(row) * kv_heads);
+    const int pos = positions[row], entry = row_entry[row];
+    int page = -1;
+    const int block = pos / page_tokens, token = pos - block * page_tokens;
+    if (pos >= 0 && entry >= 0 && entry < entries) page = mapped_page(block_table + static_cast<long>(entry) * max_blocks, block, max_blocks, pools.pages);
+    uint4 k = {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu}, v = k;
+    if (page >= 0) {
+        const long place = static_cast<long>(page) * kv_heads + kvh;
+        const long code_base = place * four_bit_codes(page_tokens, dim), power_base = place * four_bit_powers(page_tokens, dim);
+        const unsigned k_codes = *reinterpret_cast<const unsigned*>(pools.k_codes + code_base + four_bit_key(token, eight / 4, page_tokens) + eight % 4 * 4);
+        const unsigned v_codes = *reinterpret_cast<const unsigned*>(pools.v_codes + code_base + four_bit_value(token, eight, dim));
+        const float kp = power_of(pools.k_powers[power_base + four_bit_key_power(token, eight / 4, dim)]);
+        const float vp = power_of(pools.v_powers[power_base + four_bit_value_power(token, eight / 4, dim)]);
+        k = uint4{two_bf16<0>(k_codes, kp), two_bf16<1>(k_codes, kp), two_bf16<2>(k_codes, kp), two_bf16<3>(k_codes, kp)};
+        v = uint4{two_bf16<0>(v_codes, vp), two_bf16<1>(v_codes, vp), two_bf16<2>(v_codes, vp), two_bf16<3>(v_codes, vp)};
+    }
+    const long to = head_row * dim + eight * 8;
+    *reinterpret_cast<uint4*>(k_out + to) = k;
+    *reinterpret_cast<uint4*>(v_out + to) = v;
+}
+
+template <typename TIn, typename T>
+static void launch_fill(const void* qkv, void* q_out, const FourBitPools& pools, AnyVec q_gain, AnyVec k_gain, const int* positions,
+                        const int* row_entry, const int* block_table, const FillShape& s, hipStream_t stream) {
+    const int span = s.dim <= 32 ? 4 : s.dim <= 64 ? 8 : s.dim <= 128 ? 16 : 32;
+    const long waves = static_cast<long>(ceil_div(s.rows, kWave / span)) * (s.q_heads + 2 * s.kv_heads);
+    const int blocks = ceil_div(waves, kFillThreads / kWave);
+#define LEONE_FILL(SPAN)                                                                                                                    \
+    case SPAN:                                                                                                                              \
+        four_bit_fill_kernel<SPAN, TIn, T><<<blocks, kFillThreads, 0, stream>>>(static_cast<const TIn*>(qkv), static_cast<T*>(q_out), pools, \
+                                                                               q_gain, k_gain, positions, row_entry, block_table, s);      \
+        break;
+    switch (span) { LEONE_FILL(4) LEONE_FILL(8) LEONE_FILL(16) LEONE_FILL(32) }
+#undef LEONE_FILL
+}
+
+}  // namespace leone
+
+using namespace leone;
+
+extern "C" int leone_four_bit_fill(const void* qkv, int qkv_dtype, int qkv_planes, long qkv_plane, long row_width, void* q_out, int dtype,
+                                   void* k_codes, void* k_powers, void* v_codes, void* v_powers, int pages, const void* q_gain,
+                                   const void* k_gain, int gain_dtype, float eps, const float* cos_table, const float* sin_table,
+                                   int table_positions, int rotary_dim, int pairing, const int* positions, const int* row_entry,
+                                   const int* block_table, int max_blocks, int entries, int rows, int q_heads, int kv_heads, int head_dim,
+                                   int page_tokens, hipStream_t stream) {
+    const char* what = "four_bit_fill";
+    const FourBitPools pools{static_cast<uint8_t*>(k_codes), static_cast<uint8_t*>(k_powers), static_cast<uint8_t*>(v_codes),
+                             static_cast<uint8_t*>(v_powers), pages};
+    if (check_four_bit(what, pools, kv_heads, head_dim, page_tokens, max_blocks)) return 1;
+    LEONE_REQUIRE(qkv && q_out && positions && row_entry && block_table, "%s: null pointer", what);
+    LEONE_REQUIRE((dtype == kF32 || dtype == kBF16) && (qkv_dtype == dtype || qkv_dtype == kF32), "%s: the input is of the queries' type or float32", what);
+    LEONE_REQUIRE(gain_dtype == kF32 || gain_dtype == kBF16, "%s: unknown type of the gains", what);
+    LEONE_REQUIRE(rows > 0 && q_heads > 0 && entries > 0, "%s: rows %d, query heads %d, entries %d must be positive", what, rows, q_heads, entries);
+    LEONE_REQUIRE(qkv_planes >= 1 && qkv_planes <= 64 && (qkv_planes == 1 || qkv_plane % 8 == 0), "%s: %d planes of input", what, qkv_planes);
+    const long width = (static_cast<long>(q_heads) + 2L * kv_heads) * head_dim;
+    LEONE_REQUIRE(row_width >= width && row_width % 8 == 0, "%s: rows of %ld elements for heads of %ld", what, row_width, width);
+    LEONE_REQUIRE((q_gain == nullptr) == (k_gain == nullptr), "%s: q and k gains come together", what);
+    LEONE_REQUIRE((cos_table == nullptr) == (sin_table == nullptr), "%s: cos and sin tables come together", what);
+    LEONE_REQUIRE(!cos_table || (table_positions > 0 && rotary_dim > 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim),
+                  "%s: tables of %d positions for a rotation of %d of %d elements", what, table_positions, rotary_dim, head_dim);
+    LEONE_REQUIRE(pairing == 0 || pairing == 1, "%s: unknown pairing %d", what, pairing);
+    LEONE_REQUIRE((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(q_gain) |
+                   reinterpret_cast<uintptr_t>(k_gain)) % 16 == 0, "%s: the projection, the queries and the gains start at multiples of 16 bytes", what);
+    LEONE_REQUIRE(static_cast<long>(rows) * (q_heads + 2L * kv_heads) < 0x7fffffffL, "%s: too many rows for one launch", what);
+    const FillShape s{rows, q_heads, kv_heads, head_dim, page_tokens, max_blocks, entries, row_width, qkv_planes, qkv_plane, eps, cos_table,
+                      sin_table, table_positions, cos_table ? rotary_dim / 2 : 0, pairing};
+    const AnyVec qg{q_gain, gain_dtype}, kg{k_gain, gain_dtype};
+    if (dtype == kF32) launch_fill<float, float>(qkv, q_out, pools, qg, kg, positions, row_entry, block_table, s, stream);
+    else if (qkv_dtype == kF32) launch_fill<float, bf16_t>(qkv, q_out, pools, qg, kg, positions, row_entry, block_table, s, stream);
+    else launch_fill<bf16_t, bf16_t>(qkv, q_out, pools, qg, kg, positions, row_entry, block_table, s, stream);
+    LEONE_LAUNCH_CHECK(what);
+    return 0;
+}
+
+extern "C" int leone_four_bit_rows(const void* k_codes, const void* k_powers, const void* v_codes, const void* v_powers, int pages,
+                                   const int* positions, const int* row_entry, const int* block_table, int max_blocks, int entries,
+                                   void* k_out, void* v_out, int rows, int kv_heads, int head_dim, int page_tokens, hipStream_t stream) {
+    const char* what = "four_bit_rows";
+    auto bytes = [](const void* p) { return const_cast<uint8_t*>(static_cast<const uint8_t*>(p)); };
+    const FourBitPools pools{bytes(k_codes), bytes(k_powers), bytes(v_codes), bytes(v_powers), pages};
+    if (check_four_bit(what, pools, kv_heads, head_dim, page_tokens, max_blocks)) return 1;
+    LEONE_REQUIRE(positions && row_entry && block_table && k_out && v_out, "%s: null pointer", what);
+    LEONE_REQUIRE(rows > 0 && entries > 0, "%s: rows %d and entries %d must be positive", what, rows, entries);
+    LEONE_REQUIRE((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16 == 0, "%s: the results start at multiples of 16 bytes", what);
+    const long items = static_cast<long>(rows) * kv_heads * (head_dim / 8);
+    LEONE_REQUIRE(items < 0x7fffffffL * kFillThreads, "%s: too many rows for one launch", what);
+    four_bit_rows_kernel<<<ceil_div(items, kFillThreads), kFillThreads, 0, stream>>>(
+        pools, positions, row_entry, block_table, max_blocks, entries, static_cast<bf16_t*>(k_out), static_cast<bf16_t*>(v_out), items, kv_heads,
+        head_dim, page_tokens);
+    LEONE_LAUNCH_CHECK(what);
+    return 0;
+}

@@ -559,4 +559,32 @@ int leone_state_chunk();
 int leone_state_slots_max();
 int leone_state_slots(const void* table, int tensors, long chunks, int move, const int* ids, const int* to, int count, void* packed,
                       long packed_bytes, hipStream_t stream);
+// ---- the cache of 4 bits an element (four_bit.h) ----------------------------------------------------------------------------
+// The four pools: key codes [pages, kv_heads, head_dim / 32, page_tokens, 16], key powers [pages, kv_heads, page_tokens,
+// head_dim / 32], value codes [pages, kv_heads, page_tokens / 4, head_dim / 8, 4, 4], value powers [pages, kv_heads, page_tokens / 4,
+// head_dim / 32, 4], bytes that start at multiples of 16.  head_dim a multiple of 32 up to 256, page_tokens one of 8 up to 4,096.
+// Block tables are [entries, max_blocks]; what names no page (below 0, or not below `pages`) is neither read nor written.
+//
+// leone_qk_norm_rope_write for such a cache: heads normed (gains may be null) and rotated (tables may be null), q to q_out, k and
+// v into the cache.  Rows of row_width elements; the projection, q_out and the gains start at multiples of 16 bytes.
+int leone_four_bit_fill(const void* qkv, int qkv_dtype, int qkv_planes, long qkv_plane, long row_width, void* q_out, int dtype,
+                        void* k_codes, void* k_powers, void* v_codes, void* v_powers, int pages, const void* q_gain, const void* k_gain,
+                        int gain_dtype, float eps, const float* cos_table, const float* sin_table, int table_positions, int rotary_dim,
+                        int pairing, const int* positions, const int* row_entry, const int* block_table, int max_blocks, int entries, int rows,
+                        int q_heads, int kv_heads, int head_dim, int page_tokens, hipStream_t stream);
+
+// What the cache holds at the rows' positions, bfloat16 [rows, kv_heads * head_dim] each; NaN where there is no page.
+int leone_four_bit_rows(const void* k_codes, const void* k_powers, const void* v_codes, const void* v_powers, int pages,
+                        const int* positions, const int* row_entry, const int* block_table, int max_blocks, int entries, void* k_out,
+                        void* v_out, int rows, int kv_heads, int head_dim, int page_tokens, hipStream_t stream);
+
+// Attention of each row over its request's cached keys (the last `window` of them; 0: all), any shape and type.  The keys of a row
+// are cut into `splits` parts (at most leone_four_bit_max_splits()); more than one need part_acc (rows * q_heads * splits * head_dim
+// floats) and part_ml (rows * q_heads * splits * 2).
+int leone_four_bit_max_splits();
+int leone_four_bit_attend_rows(const void* q, void* out, int dtype, const void* k_codes, const void* k_powers, const void* v_codes,
+                               const void* v_powers, int pages, const int* positions, const int* row_entry, const int* block_table,
+                               int max_blocks, int entries, int rows, int q_heads, int kv_heads, int head_dim, int page_tokens, float scale,
+                               int window, int splits, float* part_acc, float* part_ml, hipStream_t stream);
+
 }

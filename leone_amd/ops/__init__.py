@@ -3022,3 +3022,7 @@ def stream_join(x: torch.Tensor, terms, first: torch.Tensor, following: Optional
          _dev(following, "following rows", None, (hidden,)), _code(following, "following rows") if following is not None else F32,
          _dev(operand, "operand"), _CODES[out_dtype], n, hidden, _stream())
     return operand
+
+
+from .four_bit import (FourBitPools, attention_rows_4bit, cache_rows_4bit, four_bit_dims, four_bit_pools,  # noqa: E402
+                       four_bit_row_splits, four_bit_supported, qk_norm_rope_write_4bit)

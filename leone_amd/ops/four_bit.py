@@ -1,0 +1,179 @@
+"""The cache of 4 bits an element: what fills it, what reads it back and what attends it.
+
+A cached key or value vector is kept in blocks of 32 consecutive elements, each a number of the 4-bit floating type e2m1 times
+a power of two of the block's own (``csrc/four_bit.h`` says how they are chosen and laid out).  A cache is four byte tensors
+(``FourBitPools``); a token and kv head of ``dim`` elements take ``dim + dim / 16`` bytes, key and value together, against
+``4 * dim`` in bfloat16.  Queries, masks, block tables and results are those of the attention over a bfloat16 or float32 cache
+(``ops.attention_rows`` and its neighbours); a row that sees no key (position -1) gives zeros, a row in whose sight a place has no page
+gives NaN.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import (BF16, F32, KernelError, _CODES, _code, _dev, _rotation_shape, _stream, call, compute_units, library)
+
+BLOCK = 32                   # elements that share a power of two
+FOUR_BIT_MAX_DIM = 256
+
+
+class FourBitPools(NamedTuple):
+    """Pages of a cache of 4 bits an element: key codes ``[pages, kv_heads, dim / 32, page_tokens, 16]``, key powers ``[pages, kv_heads,
+    page_tokens, dim / 32]``, value codes ``[pages, kv_heads, page_tokens / 4, dim / 8, 4, 4]``, value powers ``[pages, kv_heads,
+    page_tokens / 4, dim / 32, 4]``, all uint8.  Any tuple of four such tensors does in its place."""
+    k_codes: torch.Tensor
+    k_powers: torch.Tensor
+    v_codes: torch.Tensor
+    v_powers: torch.Tensor
+
+
+def four_bit_supported(head_dim: int, page_tokens: int) -> bool:
+    """Whether a cache of 4 bits an element holds heads of this size in pages of so many tokens."""
+    return head_dim % BLOCK == 0 and BLOCK <= head_dim <= FOUR_BIT_MAX_DIM and page_tokens % 8 == 0 and 8 <= page_tokens <= 4096
+
+
+def four_bit_pools(pages: int, kv_heads: int, head_dim: int, page_tokens: int, device) -> FourBitPools:
+    """A cache of zeros."""
+    if not four_bit_supported(head_dim, page_tokens):
+        raise KernelError(f"a cache of 4 bits an element takes heads of a multiple of {BLOCK} elements up to {FOUR_BIT_MAX_DIM} in pages of a "
+                          f"multiple of 8 tokens, not heads of {head_dim} in pages of {page_tokens}")
+    shapes = ((pages, kv_heads, head_dim // BLOCK, page_tokens, 16), (pages, kv_heads, page_tokens, head_dim // BLOCK),
+              (pages, kv_heads, page_tokens // 4, head_dim // 8, 4, 4), (pages, kv_heads, page_tokens // 4, head_dim // BLOCK, 4))
+    return FourBitPools(*(torch.zeros(shape, dtype=torch.uint8, device=device) for shape in shapes))
+
+
+def four_bit_dims(pools) -> tuple:
+    """(pages, kv_heads, page_tokens, head_dim) of a cache of 4 bits an element."""
+    if len(pools) != 4 or any(p.dim() != d for p, d in zip(pools, (5, 4, 6, 5))):
+        raise KernelError("a cache of 4 bits an element is four tensors: key codes, key powers, value codes, value powers")
+    pages, kv_heads, blocks, page_tokens, _ = pools[0].shape
+    dim = blocks * BLOCK
+    want = ((pages, kv_heads, blocks, page_tokens, 16), (pages, kv_heads, page_tokens, blocks),
+            (pages, kv_heads, page_tokens // 4, dim // 8, 4, 4), (pages, kv_heads, page_tokens // 4, blocks, 4))
+    found = tuple(tuple(p.shape) for p in pools)
+    if found != want or not four_bit_supported(dim, page_tokens):
+        raise KernelError(f"pools of shapes {found} are no cache of 4 bits an element")
+    return pages, kv_heads, page_tokens, dim
+
+
+def _pool_args(what: str, pools) -> tuple:
+    return tuple(_dev(p, f"{what}: {name}", torch.uint8) for p, name in zip(pools, FourBitPools._fields)) + (pools[0].shape[0],)
+
+
+def _row_args(what: str, rows: int, positions: torch.Tensor, row_entry: torch.Tensor, block_table: torch.Tensor) -> tuple:
+    if block_table.dim() != 2:
+        raise KernelError(f"{what}: a block table is int32 [entries, blocks]")
+    return (_dev(positions, f"{what}: positions", torch.int32, (rows,)), _dev(row_entry, f"{what}: row map", torch.int32, (rows,)),
+            _dev(block_table, f"{what}: block table", torch.int32), block_table.shape[1], block_table.shape[0])
+
+
+def _one_device(what: str, *tensors) -> None:
+    """A launch goes to the current device's stream: tensors of another device, or of several, are refused."""
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise KernelError(f"{what}: tensors on {', '.join(sorted(str(d) for d in devices))}; one device is needed")
+    device = next(iter(devices))
+    if device.type == "cuda" and device.index is not None and device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: tensors on {device}, which is not the current device")
+
+
+def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_heads: int, kv_heads: int, head_dim: int, q_gain: Optional[torch.Tensor],
+                            k_gain: Optional[torch.Tensor], eps: float, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+                            positions: torch.Tensor, row_entry: torch.Tensor, block_table: torch.Tensor, pools,
+                            out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                            pairing: str = "half_split") -> torch.Tensor:
+    """``qk_norm_rope_write`` for a cache of 4 bits an element: splits the fused projection, normalises and rotates q and k heads, writes
+    k and v into the cache and returns q.  ``qkv`` is ``[rows, width]`` of q's type, or float32 (also as planes ``[p, rows, width]``
+    whose sum is meant) with ``out_dtype`` naming the type of q.  Queries are rounded once, to that type; keys are computed in 64
+    bits up to their codes.  Rows at a position below 0, and rows whose place has no page, write nothing."""
+    what = "qk_norm_rope_write_4bit"
+    planes = qkv.shape[0] if qkv.dim() == 3 else 1
+    if qkv.dim() not in (2, 3) or qkv.shape[-1] != (q_heads + 2 * kv_heads) * head_dim or planes < 1:
+        raise KernelError(f"{what}: a projection {tuple(qkv.shape)} is not ({q_heads}+2*{kv_heads})*{head_dim} wide")
+    rows, width = qkv.shape[-2:]
+    kind = out_dtype or qkv.dtype
+    if kind not in _CODES or (qkv.dtype != kind and qkv.dtype != torch.float32):
+        raise KernelError(f"{what}: input {qkv.dtype} for outputs of {kind}")
+    pages, pool_heads, page_tokens, pool_dim = four_bit_dims(pools)
+    if (pool_heads, pool_dim) != (kv_heads, head_dim):
+        raise KernelError(f"{what}: a cache of {pool_heads} heads of {pool_dim} does not fit {kv_heads} heads of {head_dim}")
+    table_positions, rotary_dim, pairing_code = _rotation_shape(what, head_dim, cos, sin, pairing)
+    if (q_gain is None) != (k_gain is None) or (q_gain is not None and k_gain.dtype != q_gain.dtype):
+        raise KernelError(f"{what}: q and k gains must come together in one type")
+    if out is None:
+        out = torch.empty((rows, q_heads * head_dim), dtype=kind, device=qkv.device)
+    args = (_dev(qkv, f"{what}: qkv"), _code(qkv, what), planes, rows * width, width, _dev(out, f"{what}: q out", kind, (rows, q_heads * head_dim)),
+            _CODES[kind], *_pool_args(what, pools), _dev(q_gain, f"{what}: q gain", None, (head_dim,)),
+            _dev(k_gain, f"{what}: k gain", None, (head_dim,)), _code(q_gain, f"{what}: gain") if q_gain is not None else F32, float(eps),
+            _dev(cos, f"{what}: cos", torch.float32), _dev(sin, f"{what}: sin", torch.float32), table_positions, rotary_dim, pairing_code,
+            *_row_args(what, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, head_dim, page_tokens)
+    _one_device(what, qkv, out, *pools, q_gain, k_gain, cos, sin, positions, row_entry, block_table)
+    if rows:
+        call("leone_four_bit_fill", *args, _stream())
+    return out
+
+
+def cache_rows_4bit(pools, positions: torch.Tensor, row_entry: torch.Tensor, block_table: torch.Tensor) -> tuple:
+    """The keys and values that a cache of 4 bits an element holds at the rows' positions, bfloat16 ``[rows, kv_heads * dim]`` each (a code
+    times its power is a bfloat16 as it is).  Rows without a page give NaN."""
+    what = "cache_rows_4bit"
+    pages, kv_heads, page_tokens, dim = four_bit_dims(pools)
+    rows = positions.shape[0]
+    k = torch.empty((rows, kv_heads * dim), dtype=torch.bfloat16, device=positions.device)
+    v = torch.empty_like(k)
+    args = (*_pool_args(what, pools), *_row_args(what, rows, positions, row_entry, block_table), _dev(k, what), _dev(v, what), rows, kv_heads, dim,
+            page_tokens)
+    _one_device(what, *pools, positions, row_entry, block_table)
+    if rows:
+        call("leone_four_bit_rows", *args, _stream())
+    return k, v
+
+
+def _attention_shape(what: str, q: torch.Tensor, pools, q_heads: int, window: int) -> tuple:
+    pages, kv_heads, page_tokens, dim = four_bit_dims(pools)
+    if q.dim() != 2 or q.shape[1] != q_heads * dim or q_heads <= 0 or q_heads % kv_heads:
+        raise KernelError(f"{what}: queries {tuple(q.shape)} are not {q_heads} heads of {dim} over {kv_heads} kv heads")
+    if window < 0:
+        raise KernelError(f"{what}: window {window} must not be negative")
+    return kv_heads, page_tokens, dim
+
+
+def _workspace(rows: int, q_heads: int, dim: int, splits: int, device) -> tuple:
+    """Partial results of rows whose keys are shared out, and their maxima and sums."""
+    if splits == 1:
+        return None, None
+    return (torch.empty((rows * q_heads * splits * dim,), dtype=torch.float32, device=device),
+            torch.empty((rows * q_heads * splits * 2,), dtype=torch.float32, device=device))
+
+
+def four_bit_row_splits(blocks: int, keys: int, units: int = 256) -> int:
+    """How many workgroups share a row's keys in ``attention_rows_4bit``, where ``blocks`` workgroups would have them all: as many as
+    leave none of the chip's units idle, but no fewer than 64 keys for each of a workgroup's four waves."""
+    return max(1, min(units // max(1, blocks), keys // 256, 64))
+
+
+def attention_rows_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_entry: torch.Tensor, block_table: torch.Tensor, q_heads: int,
+                        scale: float, window: int = 0, max_context: int = 0, splits: Optional[int] = None,
+                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``attention_rows`` over a cache of 4 bits an element: any head size the cache holds, bfloat16 or float32 queries, all arithmetic in
+    float.  Each row attends its request's cached keys up to its own position (the last ``window`` of them).  ``max_context`` (0: what
+    the block table reaches) only steers into how many parts a row's keys are cut."""
+    what = "attention_rows_4bit"
+    kv_heads, page_tokens, dim = _attention_shape(what, q, pools, q_heads, window)
+    rows = q.shape[0]
+    if splits is None:
+        keys = max_context or block_table.shape[-1] * page_tokens
+        keys = min(keys, window) if window else keys
+        splits = four_bit_row_splits(rows * kv_heads * (-(-(q_heads // kv_heads) // 4)), keys, compute_units(q.device))
+    if out is None:
+        out = torch.empty_like(q)
+    part_acc, part_ml = _workspace(rows, q_heads, dim, splits, q.device)
+    args = (_dev(q, f"{what}: q"), _dev(out, f"{what}: out", q.dtype, q.shape), _code(q, what), *_pool_args(what, pools),
+            *_row_args(what, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, dim, page_tokens, float(scale), int(window),
+            int(splits), _dev(part_acc, what), _dev(part_ml, what))
+    _one_device(what, q, out, *pools, positions, row_entry, block_table)
+    if rows:
+        call("leone_four_bit_attend_rows", *args, _stream())
+    return out

@@ -158,6 +158,12 @@ _PROTOTYPES = {
     "leone_time_mix_scan": [P, P, P, ctypes.c_long, P, P, c_int, P, c_int, c_int, P, ctypes.c_long, P, ctypes.c_long, P, P,
                             c_int, c_int, c_int, P],
     "leone_time_mix_read": [P, ctypes.c_long, P, P, c_int, P, ctypes.c_long, P, c_int, c_int, c_int, P],
+    "leone_four_bit_fill": [P, c_int, c_int, ctypes.c_long, ctypes.c_long, P, c_int, P, P, P, P, c_int, P, P, c_int, c_float, P, P, c_int, c_int,
+                            c_int, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P],
+    "leone_four_bit_rows": [P, P, P, P, c_int, P, P, P, c_int, c_int, P, P, c_int, c_int, c_int, c_int, P],
+    "leone_four_bit_max_splits": [],
+    "leone_four_bit_attend_rows": [P, P, c_int, P, P, P, P, c_int, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
+                                   P, P, P],
     "leone_delta_chain": [P, c_int, P, ctypes.c_long, P, P, ctypes.c_long, c_int, c_int, c_int, c_int, P],
 }
 

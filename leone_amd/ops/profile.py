@@ -99,6 +99,9 @@ OPERATIONS = {
     "leone_bias_span_norm": "bias span norm",
     "leone_bias_glu": "swiglu",
     "leone_add_bias": "bias",
+    "leone_four_bit_fill": "qknorm rope kv",
+    "leone_four_bit_rows": "cache rows",
+    "leone_four_bit_attend_rows": "attention",
 }
 LIBRARY_PRODUCT = "gemm library"
 ORDER = ["embed", "norm", "gemv fused", "gemm rows", "gemm many", LIBRARY_PRODUCT, "gemm f32", "qknorm rope kv", "attention", "swiglu",

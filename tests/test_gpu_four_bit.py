@@ -1,0 +1,265 @@
+"""The operators of a cache of 4 bits an element against 64 bits."""
+import math
+
+import pytest
+import torch
+
+from leone_amd import ops
+from leone_amd.ops.library import KernelError
+from tests.four_bit_util import attended, held, pools_of, quantised
+
+pytestmark = pytest.mark.gpu
+DEVICE = "cuda:0"
+
+
+def _generator(seed):
+    return torch.Generator(device=DEVICE).manual_seed(seed)
+
+
+def _normal(gen, *shape):
+    return torch.randn(shape, generator=gen, device=DEVICE)
+
+
+def _tables(requests, page, gen, spare=2):
+    """Block tables of requests that hold so many tokens, pages in no order, and the number of pages."""
+    blocks = [-(-n // page) for n in requests]
+    order = torch.randperm(sum(blocks) + spare, generator=gen, device=DEVICE).int()
+    table = torch.full((len(requests), max(1, max(blocks))), -1, dtype=torch.int32, device=DEVICE)
+    at = 0
+    for i, b in enumerate(blocks):
+        table[i, :b] = order[at:at + b]
+        at += b
+    return table, sum(blocks) + spare
+
+
+def _rows(requests):
+    """positions and entries of rows given as [(first position, count)]."""
+    positions = torch.cat([torch.arange(start, start + count) for start, count in requests]).int().to(DEVICE)
+    entries = torch.cat([torch.full((count,), i) for i, (_, count) in enumerate(requests)]).int().to(DEVICE)
+    return positions, entries
+
+
+# ---- filling ---------------------------------------------------------------------------------------------------------------
+def _turned(x, cos, sin, pairing):
+    half = cos.shape[1]
+    out = x.clone()
+    i = torch.arange(half, device=x.device)
+    a, b = (2 * i, 2 * i + 1) if pairing == "adjacent" else (i, i + half)
+    c, s = cos[:, None, :].double(), sin[:, None, :].double()
+    out[..., a], out[..., b] = x[..., a] * c - x[..., b] * s, x[..., a] * s + x[..., b] * c
+    return out
+
+
+@pytest.mark.parametrize("requests,q_heads,kv_heads,dim,page,dtype,planes,norm,rotary,pairing", [
+    ([(0, 1)], 4, 2, 128, 64, torch.bfloat16, 0, True, 128, "half_split"),
+    ([(61, 7)], 4, 1, 128, 64, torch.bfloat16, 0, True, 128, "half_split"),             # over a page's edge
+    ([(5, 1), (0, 1), (200, 1), (63, 1), (64, 1)], 8, 2, 128, 16, torch.bfloat16, 2, True, 128, "half_split"),
+    ([(0, 130), (17, 33)], 2, 2, 64, 32, torch.float32, 0, True, 64, "half_split"),
+    ([(3, 19)], 3, 3, 96, 8, torch.float32, 0, True, 32, "adjacent"),
+    ([(3, 19)], 6, 2, 32, 24, torch.bfloat16, 3, False, 20, "half_split"),              # partners eight elements do not line up with
+    ([(1, 9)], 2, 1, 256, 64, torch.bfloat16, 1, True, 0, "half_split"),                # no rotation
+    ([(0, 5)], 2, 1, 160, 64, torch.bfloat16, 0, True, 160, "adjacent"),
+    ([(0, 3)], 2, 1, 224, 64, torch.float32, 0, False, 96, "half_split"),
+])
+def test_filling(requests, q_heads, kv_heads, dim, page, dtype, planes, norm, rotary, pairing):
+    gen = _generator(len(requests) * 1000 + dim + planes)
+    rows = sum(count for _, count in requests)
+    width = (q_heads + 2 * kv_heads) * dim
+    table, pages = _tables([start + count for start, count in requests], page, gen)
+    positions, entries = _rows(requests)
+    qkv = _normal(gen, max(planes, 1), rows, width) * torch.exp(_normal(gen, dim)).repeat(width // dim)
+    qkv = qkv if planes else qkv[0].to(dtype)
+    gains = [(1 + 0.2 * _normal(gen, dim)).to(dtype) for _ in range(2)] if norm else [None, None]
+    cos = sin = None
+    if rotary:
+        angles = torch.outer(torch.arange(300, device=DEVICE).double(), 1e4 ** (-torch.arange(0, rotary, 2, device=DEVICE).double() / rotary))
+        cos, sin = angles.cos().float(), angles.sin().float()
+    before = [torch.randint(0, 255, p.shape, generator=gen, device=DEVICE).to(torch.uint8) for p in ops.four_bit_pools(pages, kv_heads, dim, page, DEVICE)]
+    pools = ops.FourBitPools(*(p.clone() for p in before))
+    q = ops.qk_norm_rope_write_4bit(qkv, q_heads, kv_heads, dim, *gains, 1e-5, cos, sin, positions, entries, table, pools, out_dtype=dtype,
+                                    pairing=pairing)
+    x = (qkv.double().sum(0) if planes else qkv.double()).reshape(rows, -1, dim)
+    heads = {}
+    for name, at, count, gain in (("q", 0, q_heads, gains[0]), ("k", q_heads, kv_heads, gains[1]), ("v", q_heads + kv_heads, kv_heads, None)):
+        y = x[:, at:at + count]
+        if gain is not None:
+            y = y / (y.square().mean(-1, keepdim=True) + 1e-5).sqrt() * gain.double()
+        heads[name] = _turned(y, cos[positions.long()], sin[positions.long()], pairing) if rotary and name != "v" else y
+    # queries: a sum of `dim` squares, a handful of products and one rotation in float, then one rounding
+    size = heads["q"].abs().amax(-1, keepdim=True)
+    off = (q.double().reshape(rows, q_heads, dim) - heads["q"]).abs()
+    assert (off <= (dim + 16) * 2.0 ** -24 * size + (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24) * heads["q"].abs()).all()
+    # keys and values: the very numbers
+    k, v = ops.cache_rows_4bit(pools, positions, entries, table)
+    want_k, want_v = quantised(heads["k"]), quantised(heads["v"])
+    assert torch.equal(k.double().reshape(rows, kv_heads, dim), want_k) and torch.equal(v.double().reshape(rows, kv_heads, dim), want_v)
+    for row in {0, rows // 2, rows - 1}:
+        page_id, token = int(table[int(entries[row]), int(positions[row]) // page]), int(positions[row]) % page
+        for h in range(kv_heads):
+            key, value = held(pools, page_id, h, token)
+            assert torch.equal(key, want_k[row, h]) and torch.equal(value, want_v[row, h])
+    # every place that is no row's is left as it was
+    mine = torch.zeros(pages, page, dtype=torch.bool, device=DEVICE)
+    mine[table[entries.long(), (positions // page).long()].long(), (positions % page).long()] = True
+    for name, now, then in zip(ops.FourBitPools._fields, pools, before):
+        changed = now != then
+        if name == "k_codes":
+            changed = changed.any(-1).any(2).any(1)
+        elif name == "k_powers":
+            changed = changed.any(-1).any(1)
+        elif name == "v_codes":
+            changed = changed.any(-1).any(3).any(1).reshape(pages, page)
+        else:
+            changed = changed.any(3).any(1).reshape(pages, page)
+        assert not (changed & ~mine).any(), name
+
+
+def test_blocks_at_the_borders():
+    """Ties, zeros, the largest and smallest blocks, infinities and NaN, as values (which are only scaled)."""
+    dim, page = 32, 8
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0, 6.0, -0.25, -0.75, -5.0, -7.0, 0.0] + [0.1] * 18)
+    rows = [ties, ties * 2.0 ** 100, ties * 2.0 ** -100, torch.zeros(32), torch.full((32,), 2.0 ** -133), ties * 7.5 / 7, torch.nextafter(ties, ties * 2),
+            torch.tensor([math.inf] + [1.0] * 31), torch.tensor([1.0] * 31 + [math.nan]), torch.full((32,), -3.0e38)]
+    x = torch.stack(rows).to(DEVICE)
+    n = x.shape[0]
+    qkv = torch.cat([torch.ones(n, 2 * dim, device=DEVICE), x], dim=1)
+    positions, entries = _rows([(0, n)])
+    table, pages = _tables([n], page, _generator(3))
+    pools = ops.four_bit_pools(pages, 1, dim, page, DEVICE)
+    ops.qk_norm_rope_write_4bit(qkv, 1, 1, dim, None, None, 1e-6, None, None, positions, entries, table, pools)
+    _, v = ops.cache_rows_4bit(pools, positions, entries, table)
+    want = quantised(x).to(torch.bfloat16)
+    assert torch.equal(torch.isnan(v), torch.isnan(want)) and torch.equal(torch.nan_to_num(v), torch.nan_to_num(want))
+    assert torch.isnan(v[7]).all() and torch.isnan(v[8]).all()
+
+
+def test_rows_without_a_place():
+    """Rows at position -1, of an entry or a block that does not exist, or with a table entry that is no page, write nothing and read NaN."""
+    dim, page = 64, 16
+    table = torch.tensor([[0, -1, 99]], dtype=torch.int32, device=DEVICE)
+    positions = torch.tensor([3, 20, 40, 60, -1, 2], dtype=torch.int32, device=DEVICE)
+    entries = torch.tensor([0, 0, 0, 0, 0, 7], dtype=torch.int32, device=DEVICE)
+    pools = ops.four_bit_pools(1, 2, dim, page, DEVICE)
+    qkv = _normal(_generator(1), 6, 6 * dim).to(torch.bfloat16)
+    ops.qk_norm_rope_write_4bit(qkv, 2, 2, dim, None, None, 1e-6, None, None, positions, entries, table, pools)
+    k, v = ops.cache_rows_4bit(pools, positions, entries, table)
+    assert torch.isfinite(k[0]).all() and torch.isnan(k[1:]).all() and torch.isnan(v[1:]).all()
+    assert (pools.k_codes[:, :, :, :3] == 0).all() and (pools.k_codes[:, :, :, 4:] == 0).all()
+
+
+# ---- attention -------------------------------------------------------------------------------------------------------------
+def _cache(gen, requests, kv_heads, dim, page, spread=1.0):
+    """Pools and, by request, the keys and values they hold ``[tokens, kv_heads, dim]``; every other place holds bytes of any kind."""
+    table, pages = _tables(requests, page, gen)
+    k = quantised(_normal(gen, pages, kv_heads, page, dim) * torch.exp(0.5 * _normal(gen, dim)) * spread)
+    v = quantised(_normal(gen, pages, kv_heads, page, dim) * torch.exp(0.5 * _normal(gen, dim)))
+    pools = [p.to(DEVICE) for p in pools_of(k, v)]
+    lists = []
+    for i, n in enumerate(requests):
+        places = table[i, :-(-n // page)].long()
+        lists.append(tuple(x[places].transpose(1, 2).reshape(-1, kv_heads, dim)[:n] for x in (k, v)))
+        if n % page:                                         # behind a request's last token: NaN, and codes of any kind
+            last = int(places[-1])
+            pools[1][last, :, n % page:] = 255
+            for t in range(n % page, page):
+                pools[3][last, :, t // 4, :, t % 4] = 255
+                pools[2][last, :, t // 4, :, t % 4] = 0x7f
+    return ops.FourBitPools(*pools), table, lists
+
+
+def _check(out, q, lists, positions, entries, q_heads, scale, window, matrix):
+    """``matrix``: weights rounded to bfloat16 and products of the matrix cores; else float."""
+    dim = q.shape[1] // q_heads
+    for row in range(q.shape[0]):
+        k, v = lists[int(entries[row])]
+        want, size, spread, weights, score = attended(q[row].reshape(q_heads, dim), k, v, int(positions[row]), scale, window)
+        off = (out[row].double().reshape(q_heads, dim) - want).abs()
+        n = int(positions[row]) + 1
+        # a score is a sum of dim products: off by dim half steps of float of their sizes' sum; the matrix cores line the products of
+        # a sum up with the largest and cut what is 2^-16 below it, and hold a query to 2^-21 of its row's largest element
+        score_off = score * (2.0 ** -16 + dim * 2.0 ** -21 if matrix else dim * 2.0 ** -24)
+        bound = size * (2 * score_off + (n + 16) * 2.0 ** -23)
+        if matrix:      # every weight off by up to 2^-8 of itself, independently: four times the root of the squares' sum, above and below
+            bound = bound + 4 * 2.0 ** -8 * (spread + weights * want.abs())
+        bound = bound + (2.0 ** -8 if q.dtype == torch.bfloat16 else 2.0 ** -24) * want.abs()
+        assert (off <= bound).all(), (row, float((off / bound).max()))
+
+
+ROWS = [  # requests' lengths, q_heads, kv_heads, dim, page, window, spread of the keys
+    ([1], 4, 4, 128, 64, 0, 1.0),
+    ([2, 33, 64, 65, 1], 8, 2, 128, 16, 0, 1.0),
+    ([130, 257, 500], 6, 1, 64, 32, 0, 3.0),
+    ([700, 96, 31], 10, 2, 256, 64, 0, 1.0),
+    ([300, 299, 5], 8, 2, 128, 64, 40, 2.0),
+    ([90], 40, 2, 128, 128, 0, 1.0),                          # twenty query heads a kv head
+    ([1500, 3], 16, 2, 64, 64, 1000, 1.0),
+]
+
+
+@pytest.mark.parametrize("splits", [None, 1, 3, 64])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lengths,q_heads,kv_heads,dim,page,window,spread", ROWS + [
+    ([77, 5], 4, 2, 32, 8, 0, 1.0), ([77, 129], 4, 2, 96, 24, 50, 1.0), ([40], 2, 1, 160, 64, 0, 1.0), ([40], 2, 1, 192, 64, 0, 1.0),
+    ([40], 2, 1, 224, 64, 0, 1.0)])
+def test_rows(lengths, q_heads, kv_heads, dim, page, window, spread, dtype, splits):
+    gen = _generator(sum(lengths) + dim)
+    pools, table, lists = _cache(gen, lengths, kv_heads, dim, page, spread)
+    positions, entries = _rows([(n - 1, 1) for n in lengths])
+    q = _normal(gen, len(lengths), q_heads * dim).to(dtype)
+    out = ops.attention_rows_4bit(q, pools, positions, entries, table, q_heads, dim ** -0.5, window, splits=splits)
+    _check(out, q, lists, positions, entries, q_heads, dim ** -0.5, window, False)
+
+
+@pytest.mark.parametrize("attend", [ops.attention_rows_4bit])
+@pytest.mark.parametrize("splits", [1, 4])
+def test_rows_that_see_nothing_or_nan(attend, splits):
+    gen = _generator(5)
+    pools, table, lists = _cache(gen, [300, 300], 2, 128, 64)
+    positions = torch.tensor([299, -1, 299, 120, 299], dtype=torch.int32, device=DEVICE)
+    entries = torch.tensor([0, 0, 1, 0, 9], dtype=torch.int32, device=DEVICE)
+    table[1, 2] = -1                                        # a page in sight that is not there
+    q = _normal(gen, 5, 4 * 128).to(torch.bfloat16)
+    out = attend(q, pools, positions, entries, table, 4, 128 ** -0.5, 0, max_context=300, splits=splits)
+    assert (out[1] == 0).all() and (out[4] == 0).all() and torch.isnan(out[2]).all() and torch.isfinite(out[0]).all() and torch.isfinite(out[3]).all()
+    page, token = int(table[0, 1]), 70 % 64
+    pools.k_powers[page, 1, token, 2] = 255                 # a NaN key in the sight of both rows, second kv head only
+    out = attend(q, pools, positions, entries, table, 4, 128 ** -0.5, 0, max_context=300, splits=splits)
+    for row in (0, 3):
+        assert torch.isfinite(out[row, :256]).all() and torch.isnan(out[row, 256:]).all()
+    q[0, :128] = math.nan
+    q[3, 128 * 1 + 5] = math.inf
+    out = attend(q, pools, positions, entries, table, 4, 128 ** -0.5, 0, max_context=300, splits=splits)
+    assert torch.isnan(out[0, :128]).all() and torch.isfinite(out[0, 128:256]).all()
+    assert torch.isfinite(out[3, :128]).all() and not torch.isfinite(out[3, 128:256]).any()
+
+
+def test_refusals():
+    gen = _generator(2)
+    pools, table, _ = _cache(gen, [64], 2, 64, 64)
+    positions, entries = _rows([(63, 1)])
+    q = torch.zeros(1, 4 * 64, dtype=torch.bfloat16, device=DEVICE)
+    good = dict(q=q, pools=pools, positions=positions, row_entry=entries, block_table=table, q_heads=4, scale=0.125)
+    ops.attention_rows_4bit(**good)
+    for change in (dict(q=q.half()), dict(q_heads=3), dict(positions=positions.long()), dict(pools=pools[:3]), dict(window=-1), dict(splits=0),
+                   dict(splits=65), dict(block_table=table[0]), dict(row_entry=entries.repeat(2)), dict(q=q.cpu()), dict(positions=positions.cpu()),
+                   dict(pools=(pools[0], pools[1], pools[2], pools[1])), dict(pools=tuple(p.int() for p in pools)), dict(q=q.repeat(2, 1)[:, ::2])):
+        with pytest.raises(KernelError):
+            ops.attention_rows_4bit(**{**good, **change})
+    fill = dict(qkv=torch.zeros(1, 8 * 64, dtype=torch.bfloat16, device=DEVICE), q_heads=4, kv_heads=2, head_dim=64, q_gain=None, k_gain=None, eps=1e-6,
+                cos=None, sin=None, positions=positions, row_entry=entries, block_table=table, pools=pools)
+    ops.qk_norm_rope_write_4bit(**fill)
+    ones = torch.ones(64, device=DEVICE)
+    angles = torch.zeros(64, 33, device=DEVICE)
+    for change in (dict(q_heads=3), dict(kv_heads=1), dict(q_gain=ones), dict(q_gain=ones, k_gain=ones.bfloat16()), dict(cos=angles, sin=angles),
+                   dict(pairing="odd"), dict(cos=angles[:, :32].contiguous()), dict(out_dtype=torch.float32), dict(out_dtype=torch.float16),
+                   dict(row_entry=None and entries, positions=positions[:0]), dict(q_gain=ones[:32], k_gain=ones[:32])):
+        with pytest.raises(KernelError):
+            ops.qk_norm_rope_write_4bit(**{**fill, **change})
+    for dim, page in ((48, 64), (288, 64), (64, 12), (0, 64)):
+        assert not ops.four_bit_supported(dim, page)
+        with pytest.raises(KernelError):
+            ops.four_bit_pools(2, 2, dim, page, DEVICE)
+    # no rows: nothing is launched and nothing is wrong
+    none = torch.zeros(0, dtype=torch.int32, device=DEVICE)
+    assert ops.attention_rows_4bit(q[:0], pools, none, none, table, 4, 0.125).shape == (0, 256)
+    assert ops.cache_rows_4bit(pools, none, none, table)[0].shape == (0, 128)
