@@ -29,6 +29,7 @@
 #include "score_shape.h"
 
 #include <math.h>
+#include <type_traits>
 
 namespace leone {
 
@@ -38,6 +39,10 @@ typedef __attribute__((__vector_size__(4 * sizeof(float)))) float floatx4;
 typedef int intx8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRaise = 8.0f;                     // a score this far above the reference raises it
+
+// Query heads a workgroup of the decode kernel takes: a product has sixteen columns; wide heads' sums take the room of eight.
+__host__ __device__ constexpr int decode_columns(int dim) { return dim <= 128 ? 16 : 8; }
 
 // ---- any shape and type ------------------------------------------------------------------------------------------------
 // A workgroup takes (row, kv head, up to four of its query heads, one share of the keys), a wave 64 keys at a time: a lane takes a
@@ -201,6 +206,352 @@ four_bit_attend_rows_kernel(const T* __restrict__ q, T* __restrict__ out, FourBi
     }
 }
 
+// ---- single tokens on the matrix cores -----------------------------------------------------------------------------------
+constexpr int kDecodeWaves = 4;
+constexpr int kDecodeThreads = kDecodeWaves * kWave;
+constexpr int kTileKeys = 32;
+
+__device__ inline intx8 low_half(uint4 v) { return intx8{static_cast<int>(v.x), static_cast<int>(v.y), static_cast<int>(v.z), static_cast<int>(v.w), 0, 0, 0, 0}; }
+
+// A query row as two 8-bit parts: sixteen elements a call, `unit` 2^-e with the row's largest element in [2^7, 2^8) units.  The rest is
+// at most half of the first part's last place, sixteen units: times 32 it has the same range.
+__device__ inline void two_parts(const uint4 raw[2], float unit, int high[4], int low[4]) {
+    const unsigned w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float x[4];
+        x[0] = __uint_as_float(w[2 * i] << 16) * unit, x[1] = __uint_as_float(w[2 * i] & 0xffff0000u) * unit;
+        x[2] = __uint_as_float(w[2 * i + 1] << 16) * unit, x[3] = __uint_as_float(w[2 * i + 1] & 0xffff0000u) * unit;
+        int h = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+        h = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], h, true);
+        const floatx2 a = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
+        int r = __builtin_amdgcn_cvt_pk_fp8_f32((x[0] - a[0]) * 32.f, (x[1] - a[1]) * 32.f, 0, false);
+        r = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - b[0]) * 32.f, (x[3] - b[1]) * 32.f, r, true);
+        high[i] = h, low[i] = r;
+    }
+}
+__device__ inline unsigned largest_bits(uint4 v, unsigned top) {          // of eight bfloat16, as the bits of a float
+    const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = max(max(top, w[i] & 0x7fff0000u), w[i] << 16 & 0x7fff0000u);
+    return top;
+}
+// The power byte of a row's first part, from its largest element's bits: 255 where it is no number (its scores are then NaN).
+__device__ inline int query_power(unsigned top) {
+    const int exponent = static_cast<int>(top >> 23);
+    return exponent == 0xff ? kNanPower : max(exponent - 7, 6);
+}
+__device__ inline float query_unit(int power) { return __uint_as_float(static_cast<unsigned>(254 - (power == kNanPower ? 127 : power)) << 23); }
+__device__ inline int rest_power(int power) { return power == kNanPower ? kNanPower : power - 5; }
+
+template <int kD>
+__global__ void __launch_bounds__(kDecodeThreads, kD <= 128 ? 3 : 2)
+four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, FourBitPools pools, const int* __restrict__ positions,
+                       const int* __restrict__ row_entry, const int* __restrict__ block_table, int max_blocks, int entries, int q_heads,
+                       int kv_heads, int page_shift, float to_log2, int window, int splits, float* __restrict__ part_acc,
+                       float* __restrict__ part_ml) {
+    constexpr int kCols = decode_columns(kD);
+    constexpr int kSteps = kD <= 128 ? 1 : kD / 128;              // of 128 elements
+    constexpr int kParts = kD <= 64 ? 1 : 2;                      // products a step: heads of 64 hold both parts of a query in one
+    constexpr int kVLoads = kD <= 128 ? 1 : kD / 128;             // eights a lane has of each of its tokens
+    constexpr int kOwn = kD / 16;                                 // elements a lane has of each of its tokens
+    extern __shared__ float smem[];                               // [waves][columns][kD], then maxima and sums
+
+    const int group = q_heads / kv_heads, col_tiles = (group + kCols - 1) / kCols;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+    const int c = lane & 15, g = lane >> 4;
+    const int row = blockIdx.x, kvh = blockIdx.y / col_tiles, col0 = (blockIdx.y - kvh * col_tiles) * kCols;
+    const int cols = min(kCols, group - col0), split = blockIdx.z;
+    const int entry = row_entry[row], pos = positions[row];
+    const int n = entry >= 0 && entry < entries ? pos + 1 : 0;
+    const int lo = first_key(n - 1, window, 0);
+    const int* table = block_table + static_cast<long>(entry) * max_blocks;
+    const int t_begin = lo / kTileKeys, t_end = (n + kTileKeys - 1) / kTileKeys;
+    const int share = (t_end - t_begin + splits - 1) / splits;
+    const int my_begin = t_begin + split * share, my_end = min(my_begin + share, t_end);
+    const int page_tokens = 1 << page_shift, page_mask = page_tokens - 1;
+    const long code_bytes = four_bit_codes(page_tokens, kD), power_bytes = four_bit_powers(page_tokens, kD);
+
+    // A tile: the pages of the lane's runs of eight keys (the first product's c / 4, the second's g), then its bytes.  What is not
+    // there (a key without a page, no further tile) is read from the first page and masked later.
+    struct Pages {
+        int k, v;
+    };
+    struct Tile {
+        uint4 k[2][kSteps];                                       // keys 8 (c / 4) + c % 4 and four further
+        unsigned k_power[2][kSteps];
+        uint4 v[2][kVLoads];                                      // the runs of four tokens 8 g .. + 3 and 8 g + 4 .. + 7
+        unsigned v_power[2][kVLoads];
+        Pages at;
+    };
+    const int k_run = 8 * (c >> 2), k_token = k_run + (c & 3), v_run = 8 * g;
+    const int eight = kD <= 64 ? c >> 1 : c;                      // the lane's first eight of a token's values
+    auto find = [&](int t) {
+        Pages at{-1, -1};
+        if (t < my_end) {
+            const int key0 = t * kTileKeys;
+            // (a run partly in sight counts; one wholly outside is never asked for)
+            if (key0 + k_run < n && key0 + k_run + 8 > lo) at.k = mapped_page(table, (key0 + k_run) >> page_shift, max_blocks, pools.pages);
+            if (key0 + v_run < n && key0 + v_run + 8 > lo) at.v = mapped_page(table, (key0 + v_run) >> page_shift, max_blocks, pools.pages);
+        }
+        return at;
+    };
+    auto issue = [&](int t, const Pages& at, Tile& r) {
+        r.at = at;
+        const int key0 = t * kTileKeys;
+        {
+            const long place = static_cast<long>(max(at.k, 0)) * kv_heads + kvh;
+            const int token = at.k < 0 ? 0 : (key0 + k_token) & page_mask;
+            const uint8_t* codes = pools.k_codes + place * code_bytes + four_bit_key(token, kD <= 64 ? g & 1 : g, page_tokens);
+            const uint8_t* powers = pools.k_powers + place * power_bytes + four_bit_key_power(token, kD <= 64 ? g & 1 : g, kD);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    r.k[half][s] = load_streamed16(codes + four_bit_key(4 * half, 4 * s, page_tokens));
+                    r.k_power[half][s] = powers[four_bit_key_power(4 * half, 4 * s, kD)];
+                }
+            }
+        }
+        {
+            const long place = static_cast<long>(max(at.v, 0)) * kv_heads + kvh;
+            const int token = at.v < 0 ? 0 : (key0 + v_run) & page_mask;
+            const uint8_t* codes = pools.v_codes + place * code_bytes + four_bit_value(token, eight, kD);
+            const uint8_t* powers = pools.v_powers + place * power_bytes + four_bit_value_power(token, eight / 4, kD);
+#pragma unroll
+            for (int s = 0; s < kVLoads; ++s) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    r.v[half][s] = load_streamed16(codes + four_bit_value(4 * half, 16 * s, kD));
+                    r.v_power[half][s] = *reinterpret_cast<const unsigned*>(powers + four_bit_value_power(4 * half, 4 * s, kD));
+                }
+            }
+        }
+    };
+
+    int t = my_begin + wave;
+    Pages ahead = find(t);
+
+    // The query, column c: elements 16 g .. + 15 and 64 + 16 g .. + 15 of every 128, in two parts.
+    intx8 query[kSteps][kParts];
+    int power_high, power_low;
+    {
+        const bf16_t* from = q + (static_cast<long>(row) * q_heads + kvh * group + col0 + (c < cols ? c : 0)) * kD + 16 * g;
+        constexpr int kRuns = kD <= 64 ? 1 : 2;
+        uint4 raw[kSteps][kRuns][2];
+        unsigned top = 0;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int run = 0; run < kRuns; ++run)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    raw[s][run][i] = c < cols ? *reinterpret_cast<const uint4*>(from + 128 * s + 64 * run + 8 * i) : uint4{0u, 0u, 0u, 0u};
+                    top = largest_bits(raw[s][run][i], top);
+                }
+        auto larger = [](unsigned a, unsigned b) { return max(a, b); };
+        top = join_lanes<16>(top, larger);
+        top = join_lanes<32>(top, larger);
+        const int power = query_power(top);
+        const float unit = query_unit(power);
+        power_high = power, power_low = rest_power(power);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            int high[2][4], low[2][4];
+#pragma unroll
+            for (int run = 0; run < kRuns; ++run) two_parts(raw[s][run], unit, high[run], low[run]);
+            if constexpr (kD <= 64) {
+                query[s][0] = intx8{high[0][0], high[0][1], high[0][2], high[0][3], low[0][0], low[0][1], low[0][2], low[0][3]};
+            } else {
+                query[s][0] = intx8{high[0][0], high[0][1], high[0][2], high[0][3], high[1][0], high[1][1], high[1][2], high[1][3]};
+                query[s][1] = intx8{low[0][0], low[0][1], low[0][2], low[0][3], low[1][0], low[1][1], low[1][2], low[1][3]};
+            }
+        }
+        if constexpr (kD <= 64) {
+            if (g >= 2) power_high = power_low;                   // the second two blocks are the keys against the rest
+        }
+    }
+
+    float m_ref = -INFINITY, l_run = 0.f;
+    bool unmapped = false;
+    floatx4 acc[kOwn];
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+    auto finish = [&](int tile, Tile& r) {
+        const int key0 = tile * kTileKeys, run0 = key0 + v_run;
+        const bool full = key0 >= lo && key0 + kTileKeys <= n;    // the same for the whole wave
+        // ---- scores of keys run0 .. run0 + 7 for column c
+        floatx4 s4[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            s4[half] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                s4[half] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(low_half(r.k[half][s]), query[s][0], s4[half], 4, 0, 0,
+                                                                            static_cast<int>(r.k_power[half][s]), 0, power_high);
+                if constexpr (kParts == 2)
+                    s4[half] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(low_half(r.k[half][s]), query[s][kParts - 1], s4[half], 4, 0, 0,
+                                                                                static_cast<int>(r.k_power[half][s]), 0, power_low);
+            }
+        }
+        float sc[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sc[j] = s4[j / 4][j % 4] * to_log2;
+        const bool no_page = run0 < n && run0 + 8 > lo && r.at.v < 0;
+        unmapped |= no_page;
+        if (!full || __any(no_page)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (no_page || run0 + j < lo || run0 + j >= n) sc[j] = -INFINITY;
+            // what lies in places out of sight may be anything: a power of one makes it a number
+            if (run0 < lo || run0 + 8 > n || no_page) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    unsigned out_of_sight = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int key = run0 + 4 * half + i;
+                        if (no_page || key < lo || key >= n) out_of_sight |= 0xffu << (8 * i);
+                    }
+#pragma unroll
+                    for (int s = 0; s < kVLoads; ++s) r.v_power[half][s] = (r.v_power[half][s] & ~out_of_sight) | (0x7f7f7f7fu & out_of_sight);
+                }
+            }
+        }
+        float top = sc[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[j]);
+        if (__any(top > m_ref + kRaise)) {                        // -inf + 8 is -inf: the first scores always raise
+            top = max_lanes<16>(top);
+            top = max_lanes<32>(top);
+            const float m_new = fmaxf(m_ref, ceilf(top));
+            const float keep = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_ref - m_new);
+            m_ref = m_new;
+            l_run *= keep;
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) acc[j][v] *= keep;
+        }
+        const float shift = m_ref == -INFINITY ? 0.f : m_ref;
+        bf16x8 pt;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pt[j] = static_cast<__bf16>(__builtin_amdgcn_exp2f(sc[j] - shift));
+        {
+            const uint4 packed = __builtin_bit_cast(uint4, pt);
+            const unsigned pairs[4] = {packed.x, packed.y, packed.z, packed.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pairs[i]), __builtin_bit_cast(bf16x2, 0x3f803f80u), l_run, false);
+        }
+        // ---- values: the lane's elements of its eight tokens, two elements at a time from every token, then by element
+#pragma unroll
+        for (int s = 0; s < kVLoads; ++s) {
+            unsigned words[8];
+            float power[8];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const unsigned w[4] = {r.v[half][s].x, r.v[half][s].y, r.v[half][s].z, r.v[half][s].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    words[4 * half + i] = kD <= 64 ? w[i] >> (16 * (c & 1)) : w[i];
+                    power[4 * half + i] = power_of(r.v_power[half][s] >> (8 * i) & 255u);
+                }
+            }
+            auto pair = [&](auto index) {
+                constexpr int i = decltype(index)::value;
+                unsigned two[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) two[k] = two_bf16<i>(words[k], power[k]);
+                uint4 even, odd;
+                even.x = __builtin_amdgcn_perm(two[1], two[0], 0x05040100u), odd.x = __builtin_amdgcn_perm(two[1], two[0], 0x07060302u);
+                even.y = __builtin_amdgcn_perm(two[3], two[2], 0x05040100u), odd.y = __builtin_amdgcn_perm(two[3], two[2], 0x07060302u);
+                even.z = __builtin_amdgcn_perm(two[5], two[4], 0x05040100u), odd.z = __builtin_amdgcn_perm(two[5], two[4], 0x07060302u);
+                even.w = __builtin_amdgcn_perm(two[7], two[6], 0x05040100u), odd.w = __builtin_amdgcn_perm(two[7], two[6], 0x07060302u);
+                acc[8 * s + 2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), pt, acc[8 * s + 2 * i], 0, 0, 0);
+                acc[8 * s + 2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), pt, acc[8 * s + 2 * i + 1], 0, 0, 0);
+            };
+            pair(std::integral_constant<int, 0>{});
+            pair(std::integral_constant<int, 1>{});
+            if constexpr (kD > 64) {
+                pair(std::integral_constant<int, 2>{});
+                pair(std::integral_constant<int, 3>{});
+            }
+        }
+    };
+
+    // Two tiles in turn, and the next one's pages: a wave always has loads in flight.
+    Tile one, two;
+    if (t < my_end) {
+        issue(t, ahead, one);
+        ahead = find(t + kDecodeWaves);
+        while (true) {
+            const int t1 = t + kDecodeWaves;
+            if (t1 < my_end) issue(t1, ahead, two);
+            ahead = find(t1 + kDecodeWaves);
+            finish(t, one);
+            if (t1 >= my_end) break;
+            t = t1 + kDecodeWaves;
+            if (t < my_end) issue(t, ahead, one);
+            ahead = find(t + kDecodeWaves);
+            finish(t1, two);
+            if (t >= my_end) break;
+        }
+    }
+
+    // ---- the four waves, in their order
+    float* sm_acc = smem;
+    float* sm_m = smem + kDecodeWaves * cols * kD;
+    float* sm_l = sm_m + kDecodeWaves * cols;
+    l_run = add_lanes<16>(l_run);
+    l_run = add_lanes<32>(l_run);
+    if (__any(unmapped)) l_run = __builtin_nanf("");
+    if (l_run != l_run) m_ref = fmaxf(m_ref, 0.f);                // (a result of NaN counts, whatever its maximum)
+    if (c < cols) {
+        if (g == 0) sm_m[wave * cols + c] = m_ref, sm_l[wave * cols + c] = l_run;
+        // register v of sum j is, in row 4 g + v, element j of that lane's own
+        float* to = sm_acc + (wave * cols + c) * kD;
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+            for (int j = 0; j < kOwn; j += 4) {
+                const int d = kD <= 64 ? 4 * (4 * g + v) + j : 128 * (j / 8) + 8 * (4 * g + v) + j % 8;
+                *reinterpret_cast<floatx4*>(to + d) = floatx4{acc[j][v], acc[j + 1][v], acc[j + 2][v], acc[j + 3][v]};
+            }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x * 4; i < cols * kD; i += kDecodeThreads * 4) {
+        const int col = i / kD, d = i % kD;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kDecodeWaves; ++w) top = fmaxf(top, sm_m[w * cols + col]);
+        floatx4 num = {0.f, 0.f, 0.f, 0.f};
+        float den = 0.f;
+#pragma unroll
+        for (int w = 0; w < kDecodeWaves; ++w) {
+            const float mw = sm_m[w * cols + col];
+            const float by = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - top);
+            const floatx4 part = *reinterpret_cast<const floatx4*>(&sm_acc[(w * cols + col) * kD + d]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) num[e] += part[e] * by;
+            den += sm_l[w * cols + col] * by;
+        }
+        const long row_head = static_cast<long>(row) * q_heads + kvh * group + col0 + col;
+        if (splits == 1) {
+            const float inv = top == -INFINITY ? 0.f : 1.f / den;   // a row that sees nothing: zeros
+            uint2 packed;
+            packed.x = bf16_bits_from_float(num[0] * inv) | static_cast<unsigned>(bf16_bits_from_float(num[1] * inv)) << 16;
+            packed.y = bf16_bits_from_float(num[2] * inv) | static_cast<unsigned>(bf16_bits_from_float(num[3] * inv)) << 16;
+            *reinterpret_cast<uint2*>(out + row_head * kD + d) = packed;
+        } else {
+            const long slot = row_head * splits + split;
+            *reinterpret_cast<floatx4*>(part_acc + slot * kD + d) = num;
+            if (d == 0) part_ml[2 * slot] = top, part_ml[2 * slot + 1] = den;
+        }
+    }
+}
+
 // Merges the shares of a (row, query head) in their order: sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).  A wave a row and head;
 // lane s has share s's maximum and sum.
 constexpr int kShares = kWave;
@@ -295,6 +646,43 @@ extern "C" int leone_four_bit_attend_rows(const void* q, void* out, int dtype, c
     if (splits > 1) {
         if (dtype == kF32) merge_shares<float>(part_acc, part_ml, out, rows, q_heads, head_dim, splits, stream);
         else merge_shares<bf16_t>(part_acc, part_ml, out, rows, q_heads, head_dim, splits, stream);
+        LEONE_LAUNCH_CHECK("four_bit_merge");
+    }
+    return 0;
+}
+
+extern "C" int leone_four_bit_decode(const void* q, void* out, const void* k_codes, const void* k_powers, const void* v_codes, const void* v_powers,
+                                     int pages, const int* positions, const int* row_entry, const int* block_table, int max_blocks, int entries,
+                                     int rows, int q_heads, int kv_heads, int head_dim, int page_tokens, float scale, int window, int splits,
+                                     float* part_acc, float* part_ml, hipStream_t stream) {
+    const char* what = "four_bit_decode";
+    const FourBitPools pools = read_pools(k_codes, k_powers, v_codes, v_powers, pages);
+    if (check_four_bit(what, pools, kv_heads, head_dim, page_tokens, max_blocks)) return 1;
+    LEONE_REQUIRE(q && out && positions && row_entry && block_table, "%s: null pointer", what);
+    LEONE_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "%s: heads of 64, 128 or 256 elements, not %d", what, head_dim);
+    LEONE_REQUIRE((page_tokens & (page_tokens - 1)) == 0, "%s: pages of a power of two tokens, not %d", what, page_tokens);
+    LEONE_REQUIRE(rows > 0 && entries > 0 && q_heads > 0 && q_heads % kv_heads == 0, "%s: %d rows, %d entries, %d query heads over %d kv heads", what, rows,
+                  entries, q_heads, kv_heads);
+    LEONE_REQUIRE(window >= 0 && splits >= 1 && splits <= kShares, "%s: window %d must not be negative, splits %d in 1..%d", what, window, splits, kShares);
+    LEONE_REQUIRE(splits == 1 || (part_acc && part_ml && reinterpret_cast<uintptr_t>(part_acc) % 16 == 0), "%s: %d shares need the workspace", what, splits);
+    LEONE_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 == 0, "%s: queries and results start at multiples of 16 bytes", what);
+    const int group = q_heads / kv_heads, columns = decode_columns(head_dim);
+    const long tiles = static_cast<long>(kv_heads) * ((group + columns - 1) / columns);
+    LEONE_REQUIRE(tiles <= 65535, "%s: too many heads for one launch", what);
+    const dim3 grid(rows, static_cast<unsigned>(tiles), splits);
+    const int cols = group < columns ? group : columns;
+    const size_t shared = static_cast<size_t>(kDecodeWaves) * cols * (head_dim + 2) * sizeof(float);
+    int page_shift = 0;
+    while ((1 << page_shift) < page_tokens) ++page_shift;
+    const float to_log2 = scale * kLog2e;
+#define LEONE_DECODE(D)                                                                                                                          four_bit_decode_kernel<D><<<grid, kDecodeThreads, shared, stream>>>(                                                                             static_cast<const bf16_t*>(q), static_cast<bf16_t*>(out), pools, positions, row_entry, block_table, max_blocks, entries, q_heads,            kv_heads, page_shift, to_log2, window, splits, part_acc, part_ml)
+    if (head_dim == 64) LEONE_DECODE(64);
+    else if (head_dim == 128) LEONE_DECODE(128);
+    else LEONE_DECODE(256);
+#undef LEONE_DECODE
+    LEONE_LAUNCH_CHECK(what);
+    if (splits > 1) {
+        merge_shares<bf16_t>(part_acc, part_ml, out, rows, q_heads, head_dim, splits, stream);
         LEONE_LAUNCH_CHECK("four_bit_merge");
     }
     return 0;

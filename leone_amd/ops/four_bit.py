@@ -177,3 +177,39 @@ def attention_rows_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_ent
     if rows:
         call("leone_four_bit_attend_rows", *args, _stream())
     return out
+
+
+def four_bit_decode_supported(dtype: torch.dtype, head_dim: int, page_tokens: int) -> bool:
+    """Whether ``attention_decode_4bit`` takes this case; otherwise ``attention_rows_4bit`` does."""
+    return dtype == torch.bfloat16 and head_dim in (64, 128, 256) and four_bit_supported(head_dim, page_tokens) and page_tokens & (page_tokens - 1) == 0
+
+
+def four_bit_decode_splits(blocks: int, keys: int, units: int = 256) -> int:
+    """How many workgroups share a row's keys in ``attention_decode_4bit``, where ``blocks`` workgroups would have them all."""
+    return max(1, min(2 * units // max(1, blocks), keys // 256, 64))
+
+
+def attention_decode_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_entry: torch.Tensor, block_table: torch.Tensor, q_heads: int,
+                          scale: float, window: int = 0, max_context: int = 0, splits: Optional[int] = None,
+                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``attention_decode`` over a cache of 4 bits an element: split-KV attention of single rows on the matrix cores, bfloat16
+    (``four_bit_decode_supported``).  ``max_context`` (0: what the block table reaches) only steers the number of splits."""
+    what = "attention_decode_4bit"
+    kv_heads, page_tokens, dim = _attention_shape(what, q, pools, q_heads, window)
+    if not four_bit_decode_supported(q.dtype, dim, page_tokens):
+        raise KernelError(f"{what}: {q.dtype} heads of {dim} in pages of {page_tokens} tokens (attention_rows_4bit takes those)")
+    rows, group = q.shape[0], q_heads // kv_heads
+    if splits is None:
+        keys = max_context or block_table.shape[-1] * page_tokens
+        splits = four_bit_decode_splits(rows * kv_heads * -(-group // (16 if dim <= 128 else 8)), min(keys, window) if window else keys,
+                                        compute_units(q.device))
+    if out is None:
+        out = torch.empty_like(q)
+    part_acc, part_ml = _workspace(rows, q_heads, dim, splits, q.device)
+    args = (_dev(q, f"{what}: q"), _dev(out, f"{what}: out", q.dtype, q.shape), *_pool_args(what, pools),
+            *_row_args(what, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, dim, page_tokens, float(scale), int(window),
+            int(splits), _dev(part_acc, what), _dev(part_ml, what))
+    _one_device(what, q, out, *pools, positions, row_entry, block_table)
+    if rows:
+        call("leone_four_bit_decode", *args, _stream())
+    return out

@@ -102,6 +102,7 @@ OPERATIONS = {
     "leone_four_bit_fill": "qknorm rope kv",
     "leone_four_bit_rows": "cache rows",
     "leone_four_bit_attend_rows": "attention",
+    "leone_four_bit_decode": "attention",
 }
 LIBRARY_PRODUCT = "gemm library"
 ORDER = ["embed", "norm", "gemv fused", "gemm rows", "gemm many", LIBRARY_PRODUCT, "gemm f32", "qknorm rope kv", "attention", "swiglu",

@@ -210,7 +210,18 @@ def test_rows(lengths, q_heads, kv_heads, dim, page, window, spread, dtype, spli
     _check(out, q, lists, positions, entries, q_heads, dim ** -0.5, window, False)
 
 
-@pytest.mark.parametrize("attend", [ops.attention_rows_4bit])
+@pytest.mark.parametrize("splits", [None, 1, 3, 64])
+@pytest.mark.parametrize("lengths,q_heads,kv_heads,dim,page,window,spread", ROWS)
+def test_single_tokens(lengths, q_heads, kv_heads, dim, page, window, spread, splits):
+    gen = _generator(sum(lengths) + dim + 1)
+    pools, table, lists = _cache(gen, lengths, kv_heads, dim, page, spread)
+    positions, entries = _rows([(n - 1, 1) for n in lengths])
+    q = _normal(gen, len(lengths), q_heads * dim).to(torch.bfloat16)
+    out = ops.attention_decode_4bit(q, pools, positions, entries, table, q_heads, dim ** -0.5, window, splits=splits)
+    _check(out, q, lists, positions, entries, q_heads, dim ** -0.5, window, True)
+
+
+@pytest.mark.parametrize("attend", [ops.attention_rows_4bit, ops.attention_decode_4bit])
 @pytest.mark.parametrize("splits", [1, 4])
 def test_rows_that_see_nothing_or_nan(attend, splits):
     gen = _generator(5)
