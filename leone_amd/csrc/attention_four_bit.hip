@@ -24,7 +24,7 @@
 // The reference is raised only by a score that exceeds it by more than 8 (weights stay below 2^8): no exchange between lanes
 // otherwise.
 #include "common.h"
-#include "four_bit.h"
+#include "four_bit_attend.h"
 #include "leone_hip.h"
 #include "score_shape.h"
 
@@ -33,13 +33,6 @@
 
 namespace leone {
 
-typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8;
-typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
-typedef __attribute__((__vector_size__(4 * sizeof(float)))) float floatx4;
-typedef int intx8 __attribute__((ext_vector_type(8)));
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRaise = 8.0f;                     // a score this far above the reference raises it
 
 // Query heads a workgroup of the decode kernel takes: a product has sixteen columns; wide heads' sums take the room of eight.
 __host__ __device__ constexpr int decode_columns(int dim) { return dim <= 128 ? 16 : 8; }
@@ -210,39 +203,6 @@ four_bit_attend_rows_kernel(const T* __restrict__ q, T* __restrict__ out, FourBi
 constexpr int kDecodeWaves = 4;
 constexpr int kDecodeThreads = kDecodeWaves * kWave;
 constexpr int kTileKeys = 32;
-
-__device__ inline intx8 low_half(uint4 v) { return intx8{static_cast<int>(v.x), static_cast<int>(v.y), static_cast<int>(v.z), static_cast<int>(v.w), 0, 0, 0, 0}; }
-
-// A query row as two 8-bit parts: sixteen elements a call, `unit` 2^-e with the row's largest element in [2^7, 2^8) units.  The rest is
-// at most half of the first part's last place, sixteen units: times 32 it has the same range.
-__device__ inline void two_parts(const uint4 raw[2], float unit, int high[4], int low[4]) {
-    const unsigned w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float x[4];
-        x[0] = __uint_as_float(w[2 * i] << 16) * unit, x[1] = __uint_as_float(w[2 * i] & 0xffff0000u) * unit;
-        x[2] = __uint_as_float(w[2 * i + 1] << 16) * unit, x[3] = __uint_as_float(w[2 * i + 1] & 0xffff0000u) * unit;
-        int h = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-        h = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], h, true);
-        const floatx2 a = __builtin_amdgcn_cvt_pk_f32_fp8(h, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(h, true);
-        int r = __builtin_amdgcn_cvt_pk_fp8_f32((x[0] - a[0]) * 32.f, (x[1] - a[1]) * 32.f, 0, false);
-        r = __builtin_amdgcn_cvt_pk_fp8_f32((x[2] - b[0]) * 32.f, (x[3] - b[1]) * 32.f, r, true);
-        high[i] = h, low[i] = r;
-    }
-}
-__device__ inline unsigned largest_bits(uint4 v, unsigned top) {          // of eight bfloat16, as the bits of a float
-    const unsigned w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(max(top, w[i] & 0x7fff0000u), w[i] << 16 & 0x7fff0000u);
-    return top;
-}
-// The power byte of a row's first part, from its largest element's bits: 255 where it is no number (its scores are then NaN).
-__device__ inline int query_power(unsigned top) {
-    const int exponent = static_cast<int>(top >> 23);
-    return exponent == 0xff ? kNanPower : max(exponent - 7, 6);
-}
-__device__ inline float query_unit(int power) { return __uint_as_float(static_cast<unsigned>(254 - (power == kNanPower ? 127 : power)) << 23); }
-__device__ inline int rest_power(int power) { return power == kNanPower ? kNanPower : power - 5; }
 
 template <int kD>
 __global__ void __launch_bounds__(kDecodeThreads, kD <= 128 ? 3 : 2)
@@ -552,16 +512,24 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
     }
 }
 
-// Merges the shares of a (row, query head) in their order: sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M).  A wave a row and head;
-// lane s has share s's maximum and sum.
-constexpr int kShares = kWave;
+
+
+// The merge of shares: a wave a row and head; lane s has share s's maximum and sum.
 constexpr int kMergeThreads = 256;
 
 template <typename T>
 __global__ void __launch_bounds__(kMergeThreads)
-four_bit_merge_kernel(const float* __restrict__ part_acc, const float* __restrict__ part_ml, T* __restrict__ out, long row_heads, int dim, int splits) {
-    const long row_head = static_cast<long>(blockIdx.x) * (kMergeThreads / kWave) + threadIdx.x / kWave;
-    if (row_head >= row_heads) return;
+four_bit_merge_kernel(const float* __restrict__ part_acc, const float* __restrict__ part_ml, T* __restrict__ out, long items, int q_heads, int dim,
+                      int splits, const int* __restrict__ tiles) {
+    long row_head = static_cast<long>(blockIdx.x) * (kMergeThreads / kWave) + threadIdx.x / kWave;
+    if (row_head >= items) return;
+    if (tiles != nullptr) {
+        const long place = row_head / q_heads;
+        const int* tile = tiles + 3 * (place / kTileRows);
+        const int r = static_cast<int>(place % kTileRows);
+        if (r >= tile[2]) return;
+        row_head = (static_cast<long>(tile[1]) + r) * q_heads + row_head % q_heads;
+    }
     const int lane = threadIdx.x % kWave;
     const float m = lane < splits ? part_ml[2 * (row_head * splits + lane)] : -INFINITY;
     const float l = lane < splits ? part_ml[2 * (row_head * splits + lane) + 1] : 0.f;
@@ -591,16 +559,14 @@ four_bit_merge_kernel(const float* __restrict__ part_acc, const float* __restric
     for (int e = 0; e < 4; ++e) to[e] = from_float<T>(top == -INFINITY ? 0.f : num[e] / den);
 }
 
-template <typename T>
-static void merge_shares(const float* part_acc, const float* part_ml, void* out, int rows, int q_heads, int dim, int splits, hipStream_t stream) {
-    const long row_heads = static_cast<long>(rows) * q_heads;
-    four_bit_merge_kernel<T><<<ceil_div(row_heads, kMergeThreads / kWave), kMergeThreads, 0, stream>>>(part_acc, part_ml, static_cast<T*>(out), row_heads,
-                                                                                                      dim, splits);
-}
-
-static FourBitPools read_pools(const void* k_codes, const void* k_powers, const void* v_codes, const void* v_powers, int pages) {
-    auto bytes = [](const void* p) { return const_cast<uint8_t*>(static_cast<const uint8_t*>(p)); };
-    return FourBitPools{bytes(k_codes), bytes(k_powers), bytes(v_codes), bytes(v_powers), pages};
+void merge_four_bit_shares(const float* part_acc, const float* part_ml, void* out, int dtype, long rows, int q_heads, int dim, int splits,
+                           const int* tiles, hipStream_t stream) {
+    const long items = rows * q_heads;
+    const int blocks = ceil_div(items, kMergeThreads / kWave);
+    if (dtype == kF32)
+        four_bit_merge_kernel<float><<<blocks, kMergeThreads, 0, stream>>>(part_acc, part_ml, static_cast<float*>(out), items, q_heads, dim, splits, tiles);
+    else
+        four_bit_merge_kernel<bf16_t><<<blocks, kMergeThreads, 0, stream>>>(part_acc, part_ml, static_cast<bf16_t*>(out), items, q_heads, dim, splits, tiles);
 }
 
 }  // namespace leone
@@ -644,8 +610,7 @@ extern "C" int leone_four_bit_attend_rows(const void* q, void* out, int dtype, c
 #undef LEONE_ROWS
     LEONE_LAUNCH_CHECK(what);
     if (splits > 1) {
-        if (dtype == kF32) merge_shares<float>(part_acc, part_ml, out, rows, q_heads, head_dim, splits, stream);
-        else merge_shares<bf16_t>(part_acc, part_ml, out, rows, q_heads, head_dim, splits, stream);
+        merge_four_bit_shares(part_acc, part_ml, out, dtype, rows, q_heads, head_dim, splits, nullptr, stream);
         LEONE_LAUNCH_CHECK("four_bit_merge");
     }
     return 0;
@@ -682,7 +647,7 @@ extern "C" int leone_four_bit_decode(const void* q, void* out, const void* k_cod
 #undef LEONE_DECODE
     LEONE_LAUNCH_CHECK(what);
     if (splits > 1) {
-        merge_shares<bf16_t>(part_acc, part_ml, out, rows, q_heads, head_dim, splits, stream);
+        merge_four_bit_shares(part_acc, part_ml, out, kBF16, rows, q_heads, head_dim, splits, nullptr, stream);
         LEONE_LAUNCH_CHECK("four_bit_merge");
     }
     return 0;

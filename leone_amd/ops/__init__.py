@@ -3024,6 +3024,6 @@ def stream_join(x: torch.Tensor, terms, first: torch.Tensor, following: Optional
     return operand
 
 
-from .four_bit import (FourBitPools, attention_decode_4bit, attention_rows_4bit, cache_rows_4bit, four_bit_decode_splits,  # noqa: E402
-                       four_bit_decode_supported, four_bit_dims, four_bit_pools, four_bit_row_splits, four_bit_supported,
-                       qk_norm_rope_write_4bit)
+from .four_bit import (FourBitPools, attention_decode_4bit, attention_prefill_4bit, attention_rows_4bit, cache_rows_4bit,  # noqa: E402
+                       four_bit_decode_splits, four_bit_decode_supported, four_bit_dims, four_bit_pools, four_bit_prefill_supported,
+                       four_bit_row_splits, four_bit_supported, qk_norm_rope_write_4bit)

@@ -13,7 +13,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import (BF16, F32, KernelError, _CODES, _code, _dev, _rotation_shape, _stream, call, compute_units, library)
+from . import (F32, PREFILL_GROUP_TILES, KernelError, _CODES, _code, _dev, _rotation_shape, _stream, call, choose_prefill_splits, compute_units)
 
 BLOCK = 32                   # elements that share a power of two
 FOUR_BIT_MAX_DIM = 256
@@ -212,4 +212,40 @@ def attention_decode_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_e
     _one_device(what, q, out, *pools, positions, row_entry, block_table)
     if rows:
         call("leone_four_bit_decode", *args, _stream())
+    return out
+
+
+def four_bit_prefill_supported(dtype: torch.dtype, head_dim: int, page_tokens: int) -> bool:
+    """Whether ``attention_prefill_4bit`` takes this case; otherwise the portion's rows go through the kernels for single rows."""
+    return head_dim <= 128 and four_bit_decode_supported(dtype, head_dim, page_tokens)
+
+
+def attention_prefill_4bit(q: torch.Tensor, out: torch.Tensor, pools, positions: torch.Tensor, tiles: torch.Tensor, block_table: torch.Tensor,
+                           q_heads: int, scale: float, window: int = 0, mean_keys: int = 1, splits: Optional[int] = None,
+                           covered_rows: Optional[int] = None) -> torch.Tensor:
+    """``attention_prefill`` over a cache of 4 bits an element (``four_bit_prefill_supported``): attention for the rows that ``tiles``
+    covers, into ``out``; other rows of ``out`` are left as they are.  ``tiles``, ``mean_keys`` and ``covered_rows`` as there.  A key in
+    sight of a group of tiles whose place has no page makes the group's rows NaN."""
+    what = "attention_prefill_4bit"
+    kv_heads, page_tokens, dim = _attention_shape(what, q, pools, q_heads, window)
+    if not four_bit_prefill_supported(q.dtype, dim, page_tokens):
+        raise KernelError(f"{what}: {q.dtype} heads of {dim} in pages of {page_tokens} tokens (attention_decode_4bit and attention_rows_4bit take those)")
+    if tiles.dim() != 2 or tiles.shape[1] != 3 or tiles.shape[0] % PREFILL_GROUP_TILES:
+        raise KernelError(f"{what}: tiles must be int32 [n, 3] with n a multiple of {PREFILL_GROUP_TILES}")
+    if block_table.dim() != 2:
+        raise KernelError(f"{what}: a block table is int32 [entries, blocks]")
+    rows, groups = q.shape[0], tiles.shape[0] // PREFILL_GROUP_TILES
+    if splits is None:
+        splits = choose_prefill_splits(groups, q_heads, mean_keys, window, compute_units(q.device))
+    covered = rows if covered_rows is None else covered_rows
+    if not 0 <= covered <= rows:
+        raise KernelError(f"{what}: {covered} covered rows of {rows}")
+    part_acc, part_ml = _workspace(covered, q_heads, dim, splits, q.device)
+    args = (_dev(q, f"{what}: q"), _dev(out, f"{what}: out", q.dtype, q.shape), *_pool_args(what, pools),
+            _dev(positions, f"{what}: positions", torch.int32, (rows,)), _dev(tiles, f"{what}: tiles", torch.int32), groups,
+            _dev(block_table, f"{what}: block table", torch.int32), block_table.shape[1], block_table.shape[0], q_heads, kv_heads, dim, page_tokens,
+            float(scale), int(window), int(splits), _dev(part_acc, what), _dev(part_ml, what))
+    _one_device(what, q, out, *pools, positions, tiles, block_table)
+    if groups and covered:
+        call("leone_four_bit_prefill", *args, _stream())
     return out

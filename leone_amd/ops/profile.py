@@ -103,6 +103,7 @@ OPERATIONS = {
     "leone_four_bit_rows": "cache rows",
     "leone_four_bit_attend_rows": "attention",
     "leone_four_bit_decode": "attention",
+    "leone_four_bit_prefill": "attention",
 }
 LIBRARY_PRODUCT = "gemm library"
 ORDER = ["embed", "norm", "gemv fused", "gemm rows", "gemm many", LIBRARY_PRODUCT, "gemm f32", "qknorm rope kv", "attention", "swiglu",

@@ -244,6 +244,78 @@ def test_rows_that_see_nothing_or_nan(attend, splits):
     assert torch.isfinite(out[3, :128]).all() and not torch.isfinite(out[3, 128:256]).any()
 
 
+PORTIONS = [  # (tokens before, rows) of the portions, q_heads, kv_heads, dim, page, window, spread of the keys
+    ([(0, 1)], 2, 2, 128, 64, 0, 1.0),
+    ([(0, 64)], 4, 1, 64, 64, 0, 2.0),
+    ([(0, 200), (37, 33), (128, 128)], 4, 2, 128, 16, 0, 1.0),
+    ([(700, 129)], 8, 2, 128, 64, 0, 2.0),
+    ([(63, 65), (64, 17)], 4, 4, 64, 32, 0, 1.0),
+    ([(300, 100), (0, 150)], 4, 2, 128, 64, 50, 1.0),          # a window shorter than a stage
+    ([(5, 260)], 4, 2, 64, 128, 130, 1.0),
+    ([(3, 40)], 2, 1, 128, 8, 0, 1.0),
+]
+
+
+def _tiles(requests):
+    first, portions = 0, []
+    for i, (_, count) in enumerate(requests):
+        portions.append((i, first, count))
+        first += count
+    return ops.prefill_tiles(portions).to(DEVICE)
+
+
+@pytest.mark.parametrize("splits", [None, 1, 2, 32])
+@pytest.mark.parametrize("requests,q_heads,kv_heads,dim,page,window,spread", PORTIONS)
+def test_portions(requests, q_heads, kv_heads, dim, page, window, spread, splits):
+    lengths = [start + count for start, count in requests]
+    gen = _generator(sum(lengths) + dim + 2)
+    pools, table, lists = _cache(gen, lengths, kv_heads, dim, page, spread)
+    positions, entries = _rows(requests)
+    rows = positions.shape[0]
+    # rows behind the portions are no tile's
+    q = _normal(gen, rows + 3, q_heads * dim).to(torch.bfloat16)
+    positions = torch.cat([positions, positions.new_full((3,), 1 << 30)])
+    out = torch.full_like(q, 7.0)
+    ops.attention_prefill_4bit(q, out, pools, positions, _tiles(requests), table, q_heads, dim ** -0.5, window, mean_keys=sum(lengths), splits=splits,
+                               covered_rows=rows)
+    _check(out[:rows], q[:rows], lists, positions, entries, q_heads, dim ** -0.5, window, True)
+    assert (out[rows:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_portions_that_see_nan_or_no_page(splits, dim):
+    gen = _generator(11)
+    pools, table, lists = _cache(gen, [150, 150, 150], 2, dim, 64)
+    positions, entries = _rows([(20, 130)])
+    positions, tiles = positions.repeat(3), ops.prefill_tiles([(0, 0, 130), (1, 130, 130), (9, 260, 130)]).to(DEVICE)
+    q = _normal(gen, 390, 4 * dim).to(torch.bfloat16)
+    run = lambda: ops.attention_prefill_4bit(q, torch.zeros_like(q), pools, positions, tiles, table, 4, dim ** -0.5, splits=splits).reshape(390, 4, dim)  # noqa: E731
+    before = run()
+    assert torch.isfinite(before).all() and (before[260:] == 0).all()          # an entry that is not there sees nothing
+    # a NaN value block at key 70 counts for the rows from there on, of its kv head, in its elements
+    page, token = int(table[0, 1]), 70 % 64
+    pools.v_powers[page, 1, token // 4, 1, token % 4] = 255
+    out = run()
+    assert torch.isnan(out[50:130, 2:, 32:64]).all()
+    out[50:130, 2:, 32:64] = before[50:130, 2:, 32:64]
+    assert torch.equal(out, before)
+    # a NaN key
+    pools.v_powers[page, 1, token // 4, 1, token % 4] = 127
+    pools.k_powers[page, 0, token, 0] = 255
+    out = run()
+    assert torch.isnan(out[50:130, :2]).all() and torch.isfinite(out[:50]).all() and torch.isfinite(out[50:130, 2:]).all()
+    # a query of NaN
+    pools.k_powers[page, 0, token, 0] = 127
+    q[140, 5] = math.nan
+    out = run()
+    assert torch.isnan(out[140, 0]).all() and torch.isnan(out).sum() == dim
+    # a page that is not there spoils the group's rows only
+    table[1, 2] = -1
+    out = run()
+    assert torch.isnan(out[130:258]).all() and torch.isfinite(out[:130]).all()
+
+
 def test_refusals():
     gen = _generator(2)
     pools, table, _ = _cache(gen, [64], 2, 64, 64)
