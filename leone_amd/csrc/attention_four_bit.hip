@@ -19,8 +19,9 @@
 //    that the rounding does not depend on how the keys are cut, and the sum is taken over the rounded weights.
 // Operand layouts (lane l, c = l % 16, g = l / 16), checked on the chip: 4-bit operand: row c, elements 32 g .. + 31; 8-bit operand:
 // column c, elements 16 g .. + 15 and 64 + 16 g .. + 15; a lane's power belongs to elements 32 g .. + 31 of its row or column.
-// Result: column c, rows 4 g .. + 3.  Row c of the first half of a tile is key 8 (c / 4) + c % 4, of the second four further, so
-// that a lane's scores are those of keys 8 g .. + 7 and go into the second product as they are.
+// Result: column c, rows 4 g .. + 3.  A lane's scores of a tile's two halves are those of keys 4 g .. + 3 and 16 + 4 g .. + 3: it takes
+// the values of the same keys (the second product may sum in any order), a run of four each, and the scores go into the second
+// product as they are.  Every load of a wave is then of neighbouring bytes.
 // The reference is raised only by a score that exceeds it by more than 8 (weights stay below 2^8): no exchange between lanes
 // otherwise.
 #include "common.h"
@@ -204,7 +205,7 @@ constexpr int kDecodeWaves = 4;
 constexpr int kDecodeThreads = kDecodeWaves * kWave;
 constexpr int kTileKeys = 32;
 
-template <int kD>
+template <int kD, bool kOnePage>
 __global__ void __launch_bounds__(kDecodeThreads, kD <= 128 ? 3 : 2)
 four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, FourBitPools pools, const int* __restrict__ positions,
                        const int* __restrict__ row_entry, const int* __restrict__ block_table, int max_blocks, int entries, int q_heads,
@@ -214,6 +215,7 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
     constexpr int kSteps = kD <= 128 ? 1 : kD / 128;              // of 128 elements
     constexpr int kParts = kD <= 64 ? 1 : 2;                      // products a step: heads of 64 hold both parts of a query in one
     constexpr int kVLoads = kD <= 128 ? 1 : kD / 128;             // eights a lane has of each of its tokens
+    constexpr int kDepth = kD <= 128 ? 2 : 2;
     constexpr int kOwn = kD / 16;                                 // elements a lane has of each of its tokens
     extern __shared__ float smem[];                               // [waves][columns][kD], then maxima and sums
 
@@ -223,8 +225,10 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
     const int row = blockIdx.x, kvh = blockIdx.y / col_tiles, col0 = (blockIdx.y - kvh * col_tiles) * kCols;
     const int cols = min(kCols, group - col0), split = blockIdx.z;
     const int entry = row_entry[row], pos = positions[row];
-    const int n = entry >= 0 && entry < entries ? pos + 1 : 0;
-    const int lo = first_key(n - 1, window, 0);
+    const int all = entry >= 0 && entry < entries ? pos + 1 : 0;
+    const int lo = first_key(all - 1, window, 0);
+    // keys behind the block table's reach have no page
+    const int n = all > 0 ? static_cast<int>(min(static_cast<long>(all), static_cast<long>(max_blocks) << page_shift)) : 0;
     const int* table = block_table + static_cast<long>(entry) * max_blocks;
     const int t_begin = lo / kTileKeys, t_end = (n + kTileKeys - 1) / kTileKeys;
     const int share = (t_end - t_begin + splits - 1) / splits;
@@ -232,65 +236,64 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
     const int page_tokens = 1 << page_shift, page_mask = page_tokens - 1;
     const long code_bytes = four_bit_codes(page_tokens, kD), power_bytes = four_bit_powers(page_tokens, kD);
 
-    // A tile: the pages of the lane's runs of eight keys (the first product's c / 4, the second's g), then its bytes.  What is not
-    // there (a key without a page, no further tile) is read from the first page and masked later.
-    struct Pages {
-        int k, v;
-    };
+    // A tile: the page ids of its halves of sixteen keys (of the whole tile, where pages hold 32 or more: kOnePage) come by scalar loads,
+    // which are waited for apart from the others, then its bytes.  What has no page is read from the first one and masked later.
+    // (Every call of `issue` is the same loads whatever the tile, also behind the last: after a load that may or may not have been
+    // issued the compiler waits for all.  Addresses are a base that is the same for the wave and a lane's 32-bit offset that does not
+    // change: with 64-bit products for every load a tile cost 1,700 cycles of a wave, half of it scalar arithmetic.)
+    constexpr int kPages = kOnePage ? 1 : 2;
     struct Tile {
-        uint4 k[2][kSteps];                                       // keys 8 (c / 4) + c % 4 and four further
+        uint4 k[2][kSteps];                                       // key 16 half + c
         unsigned k_power[2][kSteps];
-        uint4 v[2][kVLoads];                                      // the runs of four tokens 8 g .. + 3 and 8 g + 4 .. + 7
+        uint4 v[2][kVLoads];                                      // keys 16 half + 4 g .. + 3
         unsigned v_power[2][kVLoads];
-        Pages at;
+        int page[kPages];
     };
-    const int k_run = 8 * (c >> 2), k_token = k_run + (c & 3), v_run = 8 * g;
-    const int eight = kD <= 64 ? c >> 1 : c;                      // the lane's first eight of a token's values
+    struct Pages {
+        int id[kPages];
+    };
+    const int k_block = kD <= 64 ? g & 1 : g, eight = kD <= 64 ? c >> 1 : c;           // the lane's first block and eight
+    const unsigned k_code_at = four_bit_key(c, k_block, page_tokens), k_power_at = four_bit_key_power(c, k_block, kD);
+    const unsigned v_code_at = four_bit_value(4 * g, eight, kD), v_power_at = four_bit_value_power(4 * g, eight / 4, kD);
+    const unsigned code_stride = static_cast<unsigned>(code_bytes) * kv_heads, power_stride = static_cast<unsigned>(power_bytes) * kv_heads;
+    const uint8_t* k_codes = pools.k_codes + kvh * code_bytes;
+    const uint8_t* k_powers = pools.k_powers + kvh * power_bytes;
+    const uint8_t* v_codes = pools.v_codes + kvh * code_bytes;
+    const uint8_t* v_powers = pools.v_powers + kvh * power_bytes;
     auto find = [&](int t) {
-        Pages at{-1, -1};
-        if (t < my_end) {
-            const int key0 = t * kTileKeys;
-            // (a run partly in sight counts; one wholly outside is never asked for)
-            if (key0 + k_run < n && key0 + k_run + 8 > lo) at.k = mapped_page(table, (key0 + k_run) >> page_shift, max_blocks, pools.pages);
-            if (key0 + v_run < n && key0 + v_run + 8 > lo) at.v = mapped_page(table, (key0 + v_run) >> page_shift, max_blocks, pools.pages);
-        }
-        return at;
+        Pages found;
+#pragma unroll
+        for (int i = 0; i < kPages; ++i) found.id[i] = table[min((t * kTileKeys + 16 * i) >> page_shift, max_blocks - 1)];
+        return found;
     };
-    auto issue = [&](int t, const Pages& at, Tile& r) {
-        r.at = at;
-        const int key0 = t * kTileKeys;
-        {
-            const long place = static_cast<long>(max(at.k, 0)) * kv_heads + kvh;
-            const int token = at.k < 0 ? 0 : (key0 + k_token) & page_mask;
-            const uint8_t* codes = pools.k_codes + place * code_bytes + four_bit_key(token, kD <= 64 ? g & 1 : g, page_tokens);
-            const uint8_t* powers = pools.k_powers + place * power_bytes + four_bit_key_power(token, kD <= 64 ? g & 1 : g, kD);
+    auto issue = [&](int t, const Pages& found, Tile& r) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int i = kOnePage ? 0 : half;
+            r.page[i] = found.id[i];
+            const unsigned page = static_cast<unsigned>(found.id[i]) < static_cast<unsigned>(pools.pages) ? found.id[i] : 0;
+            const unsigned token = (t * kTileKeys + 16 * half) & page_mask;
+            const unsigned long long codes = static_cast<unsigned long long>(page) * code_stride, powers = static_cast<unsigned long long>(page) * power_stride;
+            const uint8_t* kc = k_codes + codes + 16 * token;                             // (a block of so many tokens' keys)
+            const uint8_t* kp = k_powers + powers + kD / kBlock * token;
+            const uint8_t* vc = v_codes + codes + kD / 2 * token;
+            const uint8_t* vp = v_powers + powers + kD / kBlock * token;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    r.k[half][s] = load_streamed16(codes + four_bit_key(4 * half, 4 * s, page_tokens));
-                    r.k_power[half][s] = powers[four_bit_key_power(4 * half, 4 * s, kD)];
-                }
+                r.k[half][s] = load_streamed16(kc + (k_code_at + s * four_bit_key(0, 4, page_tokens)));
+                r.k_power[half][s] = kp[k_power_at + 4 * s];
             }
-        }
-        {
-            const long place = static_cast<long>(max(at.v, 0)) * kv_heads + kvh;
-            const int token = at.v < 0 ? 0 : (key0 + v_run) & page_mask;
-            const uint8_t* codes = pools.v_codes + place * code_bytes + four_bit_value(token, eight, kD);
-            const uint8_t* powers = pools.v_powers + place * power_bytes + four_bit_value_power(token, eight / 4, kD);
 #pragma unroll
             for (int s = 0; s < kVLoads; ++s) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    r.v[half][s] = load_streamed16(codes + four_bit_value(4 * half, 16 * s, kD));
-                    r.v_power[half][s] = *reinterpret_cast<const unsigned*>(powers + four_bit_value_power(4 * half, 4 * s, kD));
-                }
+                r.v[half][s] = load_streamed16(vc + (v_code_at + s * four_bit_value(0, 16, kD)));
+                r.v_power[half][s] = *reinterpret_cast<const unsigned*>(vp + (v_power_at + s * four_bit_value_power(0, 4, kD)));
             }
         }
     };
 
     int t = my_begin + wave;
-    Pages ahead = find(t);
+    Pages ahead{};
+    if (t < my_end) ahead = find(t);
 
     // The query, column c: elements 16 g .. + 15 and 64 + 16 g .. + 15 of every 128, in two parts.
     intx8 query[kSteps][kParts];
@@ -333,15 +336,18 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
     }
 
     float m_ref = -INFINITY, l_run = 0.f;
-    bool unmapped = false;
+    bool unmapped = n < all;
     floatx4 acc[kOwn];
 #pragma unroll
     for (int j = 0; j < kOwn; ++j) acc[j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
     auto finish = [&](int tile, Tile& r) {
-        const int key0 = tile * kTileKeys, run0 = key0 + v_run;
-        const bool full = key0 >= lo && key0 + kTileKeys <= n;    // the same for the whole wave
-        // ---- scores of keys run0 .. run0 + 7 for column c
+        const int key0 = tile * kTileKeys;
+        bool no_page[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) no_page[half] = static_cast<unsigned>(r.page[kOnePage ? 0 : half]) >= static_cast<unsigned>(pools.pages);
+        const bool full = key0 >= lo && key0 + kTileKeys <= n && !no_page[0] && !no_page[1];      // the same for the whole wave
+        // ---- scores of keys 4 g .. + 3 of both halves for column c
         floatx4 s4[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -358,25 +364,19 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
         float sc[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) sc[j] = s4[j / 4][j % 4] * to_log2;
-        const bool no_page = run0 < n && run0 + 8 > lo && r.at.v < 0;
-        unmapped |= no_page;
-        if (!full || __any(no_page)) {
+        if (!full) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (no_page || run0 + j < lo || run0 + j >= n) sc[j] = -INFINITY;
-            // what lies in places out of sight may be anything: a power of one makes it a number
-            if (run0 < lo || run0 + 8 > n || no_page) {
+            for (int half = 0; half < 2; ++half) {
+                unmapped |= no_page[half] && key0 + 16 * half < n && key0 + 16 * half + 16 > lo;
+                unsigned hidden = 0;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    unsigned out_of_sight = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int key = run0 + 4 * half + i;
-                        if (no_page || key < lo || key >= n) out_of_sight |= 0xffu << (8 * i);
-                    }
-#pragma unroll
-                    for (int s = 0; s < kVLoads; ++s) r.v_power[half][s] = (r.v_power[half][s] & ~out_of_sight) | (0x7f7f7f7fu & out_of_sight);
+                for (int i = 0; i < 4; ++i) {
+                    const int key = key0 + 16 * half + 4 * g + i;
+                    if (no_page[half] || key < lo || key >= n) sc[4 * half + i] = -INFINITY, hidden |= 0xffu << (8 * i);
                 }
+                // what lies in places out of sight may be anything: a power of one makes it a number
+#pragma unroll
+                for (int s = 0; s < kVLoads; ++s) r.v_power[half][s] = (r.v_power[half][s] & ~hidden) | (0x7f7f7f7fu & hidden);
             }
         }
         float top = sc[0];
@@ -441,22 +441,27 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
         }
     };
 
-    // Two tiles in turn, and the next one's pages: a wave always has loads in flight.
-    Tile one, two;
+    // kDepth tiles in turn: a wave always has loads in flight.
+    Tile ring[kDepth];
     if (t < my_end) {
-        issue(t, ahead, one);
-        ahead = find(t + kDecodeWaves);
-        while (true) {
-            const int t1 = t + kDecodeWaves;
-            if (t1 < my_end) issue(t1, ahead, two);
-            ahead = find(t1 + kDecodeWaves);
-            finish(t, one);
-            if (t1 >= my_end) break;
-            t = t1 + kDecodeWaves;
-            if (t < my_end) issue(t, ahead, one);
-            ahead = find(t + kDecodeWaves);
-            finish(t1, two);
-            if (t >= my_end) break;
+#pragma unroll
+        for (int i = 0; i < kDepth - 1; ++i) {
+            issue(t + i * kDecodeWaves, ahead, ring[i]);
+            ahead = find(t + (i + 1) * kDecodeWaves);
+        }
+        bool more = true;
+        while (more) {
+#pragma unroll
+            for (int i = 0; i < kDepth; ++i) {
+                issue(t + (kDepth - 1) * kDecodeWaves, ahead, ring[(i + kDepth - 1) % kDepth]);
+                ahead = find(t + kDepth * kDecodeWaves);
+                finish(t, ring[i]);
+                t += kDecodeWaves;
+                if (t >= my_end) {
+                    more = false;
+                    break;
+                }
+            }
         }
     }
 
@@ -466,7 +471,7 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
     float* sm_l = sm_m + kDecodeWaves * cols;
     l_run = add_lanes<16>(l_run);
     l_run = add_lanes<32>(l_run);
-    if (__any(unmapped)) l_run = __builtin_nanf("");
+    if (unmapped) l_run = __builtin_nanf("");
     if (l_run != l_run) m_ref = fmaxf(m_ref, 0.f);                // (a result of NaN counts, whatever its maximum)
     if (c < cols) {
         if (g == 0) sm_m[wave * cols + c] = m_ref, sm_l[wave * cols + c] = l_run;
@@ -625,7 +630,7 @@ extern "C" int leone_four_bit_decode(const void* q, void* out, const void* k_cod
     if (check_four_bit(what, pools, kv_heads, head_dim, page_tokens, max_blocks)) return 1;
     LEONE_REQUIRE(q && out && positions && row_entry && block_table, "%s: null pointer", what);
     LEONE_REQUIRE(head_dim == 64 || head_dim == 128 || head_dim == 256, "%s: heads of 64, 128 or 256 elements, not %d", what, head_dim);
-    LEONE_REQUIRE((page_tokens & (page_tokens - 1)) == 0, "%s: pages of a power of two tokens, not %d", what, page_tokens);
+    LEONE_REQUIRE(page_tokens >= 16 && (page_tokens & (page_tokens - 1)) == 0, "%s: pages of a power of two tokens from 16 on, not %d", what, page_tokens);
     LEONE_REQUIRE(rows > 0 && entries > 0 && q_heads > 0 && q_heads % kv_heads == 0, "%s: %d rows, %d entries, %d query heads over %d kv heads", what, rows,
                   entries, q_heads, kv_heads);
     LEONE_REQUIRE(window >= 0 && splits >= 1 && splits <= kShares, "%s: window %d must not be negative, splits %d in 1..%d", what, window, splits, kShares);
@@ -634,17 +639,27 @@ extern "C" int leone_four_bit_decode(const void* q, void* out, const void* k_cod
     const int group = q_heads / kv_heads, columns = decode_columns(head_dim);
     const long tiles = static_cast<long>(kv_heads) * ((group + columns - 1) / columns);
     LEONE_REQUIRE(tiles <= 65535, "%s: too many heads for one launch", what);
+    LEONE_REQUIRE(four_bit_codes(page_tokens, head_dim) * kv_heads < 0x7fffffffL, "%s: a page of %d heads is too large", what, kv_heads);
     const dim3 grid(rows, static_cast<unsigned>(tiles), splits);
     const int cols = group < columns ? group : columns;
     const size_t shared = static_cast<size_t>(kDecodeWaves) * cols * (head_dim + 2) * sizeof(float);
     int page_shift = 0;
     while ((1 << page_shift) < page_tokens) ++page_shift;
     const float to_log2 = scale * kLog2e;
-#define LEONE_DECODE(D)                                                                                                                          four_bit_decode_kernel<D><<<grid, kDecodeThreads, shared, stream>>>(                                                                             static_cast<const bf16_t*>(q), static_cast<bf16_t*>(out), pools, positions, row_entry, block_table, max_blocks, entries, q_heads,            kv_heads, page_shift, to_log2, window, splits, part_acc, part_ml)
+#define LEONE_DECODE_CALL(D, ONE)                                                                                                          \
+    four_bit_decode_kernel<D, ONE><<<grid, kDecodeThreads, shared, stream>>>(                                                              \
+        static_cast<const bf16_t*>(q), static_cast<bf16_t*>(out), pools, positions, row_entry, block_table, max_blocks, entries, q_heads,  \
+        kv_heads, page_shift, to_log2, window, splits, part_acc, part_ml)
+#define LEONE_DECODE(D)                                           \
+    do {                                                          \
+        if (page_tokens >= kTileKeys) LEONE_DECODE_CALL(D, true); \
+        else LEONE_DECODE_CALL(D, false);                         \
+    } while (0)
     if (head_dim == 64) LEONE_DECODE(64);
     else if (head_dim == 128) LEONE_DECODE(128);
     else LEONE_DECODE(256);
 #undef LEONE_DECODE
+#undef LEONE_DECODE_CALL
     LEONE_LAUNCH_CHECK(what);
     if (splits > 1) {
         merge_four_bit_shares(part_acc, part_ml, out, kBF16, rows, q_heads, head_dim, splits, nullptr, stream);

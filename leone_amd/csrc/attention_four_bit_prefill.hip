@@ -405,7 +405,7 @@ extern "C" int leone_four_bit_prefill(const void* q, void* out, const void* k_co
     if (check_four_bit(what, pools, kv_heads, head_dim, page_tokens, max_blocks)) return 1;
     LEONE_REQUIRE(q && out && positions && tiles && block_table, "%s: null pointer", what);
     LEONE_REQUIRE(head_dim == 64 || head_dim == 128, "%s: heads of 64 or 128 elements, not %d", what, head_dim);
-    LEONE_REQUIRE((page_tokens & (page_tokens - 1)) == 0, "%s: pages of a power of two tokens, not %d", what, page_tokens);
+    LEONE_REQUIRE(page_tokens >= 16 && (page_tokens & (page_tokens - 1)) == 0, "%s: pages of a power of two tokens from 16 on, not %d", what, page_tokens);
     LEONE_REQUIRE(n_groups > 0 && entries > 0 && q_heads > 0 && q_heads % kv_heads == 0, "%s: %d tile groups, %d entries, %d query heads over %d kv heads",
                   what, n_groups, entries, q_heads, kv_heads);
     LEONE_REQUIRE(static_cast<long>(n_groups) * q_heads <= 0x7fffffffL / kTileRows, "%s: too many tile groups", what);

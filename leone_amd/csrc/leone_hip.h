@@ -587,13 +587,13 @@ int leone_four_bit_attend_rows(const void* q, void* out, int dtype, const void* 
                                int max_blocks, int entries, int rows, int q_heads, int kv_heads, int head_dim, int page_tokens, float scale,
                                int window, int splits, float* part_acc, float* part_ml, hipStream_t stream);
 
-// The same for bfloat16 queries on the matrix cores: heads of 64, 128 or 256 elements, pages of a power of two tokens.
+// The same for bfloat16 queries on the matrix cores: heads of 64, 128 or 256 elements, pages of a power of two tokens from 16 on.
 int leone_four_bit_decode(const void* q, void* out, const void* k_codes, const void* k_powers, const void* v_codes, const void* v_powers,
                           int pages, const int* positions, const int* row_entry, const int* block_table, int max_blocks, int entries,
                           int rows, int q_heads, int kv_heads, int head_dim, int page_tokens, float scale, int window, int splits,
                           float* part_acc, float* part_ml, hipStream_t stream);
 
-// leone_attention_prefill over such a cache: heads of 64 or 128 elements, pages of a power of two tokens, up to 32 ranges.  Only the rows
+// leone_attention_prefill over such a cache: heads of 64 or 128 elements, pages of a power of two tokens from 16 on, up to 32 ranges.  Only the rows
 // that a tile names are written.
 int leone_four_bit_prefill(const void* q, void* out, const void* k_codes, const void* k_powers, const void* v_codes, const void* v_powers,
                            int pages, const int* positions, const int* tiles, int n_groups, const int* block_table, int max_blocks,

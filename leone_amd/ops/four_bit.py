@@ -181,12 +181,16 @@ def attention_rows_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_ent
 
 def four_bit_decode_supported(dtype: torch.dtype, head_dim: int, page_tokens: int) -> bool:
     """Whether ``attention_decode_4bit`` takes this case; otherwise ``attention_rows_4bit`` does."""
-    return dtype == torch.bfloat16 and head_dim in (64, 128, 256) and four_bit_supported(head_dim, page_tokens) and page_tokens & (page_tokens - 1) == 0
+    return (dtype == torch.bfloat16 and head_dim in (64, 128, 256) and four_bit_supported(head_dim, page_tokens)
+            and page_tokens >= 16 and page_tokens & (page_tokens - 1) == 0)
 
 
 def four_bit_decode_splits(blocks: int, keys: int, units: int = 256) -> int:
-    """How many workgroups share a row's keys in ``attention_decode_4bit``, where ``blocks`` workgroups would have them all."""
-    return max(1, min(2 * units // max(1, blocks), keys // 256, 64))
+    """How many workgroups share a row's keys in ``attention_decode_4bit``, where ``blocks`` workgroups would have them all: two workgroups
+    for each of the chip's units, but at least 256 keys each (two tiles for each of its waves) and at most 32 to a row, whose partial
+    results the second launch reads.  us, 128 elements a head, by splits: 64 blocks of 8,192 keys 41.5 (1), 18.2 (4), 17.0 (8), 18.8 (12);
+    8 of 32,768 25.5 (8), 17.6 (16), 14.4 (32), 16.5 (64); 512 of 300 to 8,191 72.8 (1), 82.7 (2), 77.2 (4)."""
+    return max(1, min(2 * units // max(1, blocks), keys // 256, 32))
 
 
 def attention_decode_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_entry: torch.Tensor, block_table: torch.Tensor, q_heads: int,

@@ -252,7 +252,7 @@ PORTIONS = [  # (tokens before, rows) of the portions, q_heads, kv_heads, dim, p
     ([(63, 65), (64, 17)], 4, 4, 64, 32, 0, 1.0),
     ([(300, 100), (0, 150)], 4, 2, 128, 64, 50, 1.0),          # a window shorter than a stage
     ([(5, 260)], 4, 2, 64, 128, 130, 1.0),
-    ([(3, 40)], 2, 1, 128, 8, 0, 1.0),
+    ([(3, 40)], 2, 1, 128, 16, 0, 1.0),
 ]
 
 
