@@ -49,33 +49,54 @@ __device__ inline void load_eight(const TIn* __restrict__ from, int planes, long
 __device__ inline float root(float v) { return sqrtf(v); }
 __device__ inline double root(double v) { return sqrt(v); }
 
+// The value that the lane kOff further (or nearer) holds; every lane of the wave takes part.
+template <int kOff, typename T>
+__device__ inline T of_partner(T v, int lane) {
+    const Pair<T> both = lane_pair<kOff>(v);
+    if constexpr (kOff >= 16) return lane & kOff ? both.a : both.b;
+    else return both.b;
+}
+
+// How a head is rotated: not at all, whole in halves (dim a power of two: the partners are half a head's lanes away, the angles are read
+// in runs), or in any other way (partners are loaded a second time, angles one by one).
+enum Turn : int { kNoTurn = 0, kWholeHalves = 1, kAnyTurn = 2 };
+
 // Eight elements of a query or key head: normed and rotated.  `at` is the lane's first element; lanes behind the head (at >= dim)
 // take part in the sum with nothing.
-template <int kSpan, typename TIn, typename Acc>
-__device__ inline void make_eight(const TIn* __restrict__ head, int at, const FillShape& s, const AnyVec& gain, int pos, Acc x[8]) {
+template <int kSpan, int kTurn, typename TIn, typename Acc>
+__device__ inline void make_eight(const TIn* __restrict__ head, int at, int lane, const FillShape& s, const AnyVec& gain, int pos, Acc x[8]) {
     const bool in_head = at < s.dim;
+    const int half = s.rotary_half;
+    const long angles = static_cast<long>(pos < s.table_positions ? pos : s.table_positions - 1) * half;   // (the host checks the bound)
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = 0;
     if (in_head) load_eight<TIn, Acc>(head + at, s.planes, s.plane, x);
+    float g[8], c[8], n[8];
+    if (gain.ptr && in_head) load_any8(gain, at, g);
+    if constexpr (kTurn == kWholeHalves) {
+        load_any8(AnyVec{s.cos_table, kF32}, angles + (at & (half - 1)), c);
+        load_any8(AnyVec{s.sin_table, kF32}, angles + (at & (half - 1)), n);
+    }
     // the partners, where they are not among the lane's own
-    const int half = s.rotary_half;
-    const bool turned = s.cos_table != nullptr && at < 2 * half;
+    const bool turned = kTurn == kAnyTurn && at < 2 * half;
     const bool apart = turned && s.pairing == 0;
-    Acc other[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) other[i] = 0;
+    [[maybe_unused]] Acc other[8];
     auto partner = [&](int d) { return d < half ? d + half : d - half; };
-    if (apart && in_head) {
-        if (half % 8 == 0) {
-            load_eight<TIn, Acc>(head + partner(at), s.planes, s.plane, other);
-        } else {
+    if constexpr (kTurn == kAnyTurn) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (at + i < 2 * half)
-                    for (int p = 0; p < s.planes; ++p) {
-                        const TIn v = head[p * s.plane + partner(at + i)];
-                        other[i] += static_cast<Acc>(to_float(v));
-                    }
+        for (int i = 0; i < 8; ++i) other[i] = 0;
+        if (apart && in_head) {
+            if (half % 8 == 0) {
+                load_eight<TIn, Acc>(head + partner(at), s.planes, s.plane, other);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (at + i < 2 * half)
+                        for (int p = 0; p < s.planes; ++p) {
+                            const TIn v = head[p * s.plane + partner(at + i)];
+                            other[i] += static_cast<Acc>(to_float(v));
+                        }
+            }
         }
     }
     if (gain.ptr) {
@@ -85,8 +106,6 @@ __device__ inline void make_eight(const TIn* __restrict__ head, int at, const Fi
         squares = join_span<kSpan>(squares, [](Acc a, Acc b) { return a + b; });
         const Acc inv = Acc(1) / root(squares / static_cast<Acc>(s.dim) + static_cast<Acc>(s.eps));
         if (in_head) {
-            float g[8];
-            load_any8(gain, at, g);
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = x[i] * static_cast<Acc>(g[i]) * inv;
             if (apart) {
@@ -96,16 +115,23 @@ __device__ inline void make_eight(const TIn* __restrict__ head, int at, const Fi
             }
         }
     }
+    if constexpr (kTurn == kWholeHalves) {
+        const bool first = (lane & (kSpan / 2)) == 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const Acc o = of_partner<kSpan / 2>(x[i], lane), cosine = c[i], sine = first ? -n[i] : n[i];
+            x[i] = x[i] * cosine + o * sine;
+        }
+    }
     if (!turned) return;
-    const long angles = static_cast<long>(pos < s.table_positions ? pos : s.table_positions - 1) * half;   // (the host checks the bound)
     if (s.pairing != 0) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
             if (at + i >= 2 * half) continue;
-            const Acc c = s.cos_table[angles + (at + i) / 2], n = s.sin_table[angles + (at + i) / 2];
+            const Acc cosine = s.cos_table[angles + (at + i) / 2], sine = s.sin_table[angles + (at + i) / 2];
             const Acc a = x[i], b = x[i + 1];
-            x[i] = a * c - b * n;
-            x[i + 1] = a * n + b * c;
+            x[i] = a * cosine - b * sine;
+            x[i + 1] = a * sine + b * cosine;
         }
         return;
     }
@@ -114,8 +140,8 @@ __device__ inline void make_eight(const TIn* __restrict__ head, int at, const Fi
         const int d = at + i;
         if (d >= 2 * half) continue;
         const bool first = d < half;
-        const Acc c = s.cos_table[angles + (first ? d : d - half)], n = s.sin_table[angles + (first ? d : d - half)];
-        x[i] = first ? x[i] * c - other[i] * n : other[i] * n + x[i] * c;
+        const Acc cosine = s.cos_table[angles + (first ? d : d - half)], sine = s.sin_table[angles + (first ? d : d - half)];
+        x[i] = first ? x[i] * cosine - other[i] * sine : other[i] * sine + x[i] * cosine;
     }
 }
 
@@ -162,7 +188,7 @@ __device__ inline unsigned eight_codes(const Acc x[8], int& power) {
     return codes;
 }
 
-template <int kSpan, typename TIn, typename T>
+template <int kSpan, int kTurn, typename TIn, typename T>
 __global__ void __launch_bounds__(kFillThreads)
 four_bit_fill_kernel(const TIn* __restrict__ qkv, T* __restrict__ q_out, FourBitPools pools, AnyVec q_gain, AnyVec k_gain,
                      const int* __restrict__ positions, const int* __restrict__ row_entry, const int* __restrict__ block_table, FillShape s) {
@@ -180,7 +206,7 @@ four_bit_fill_kernel(const TIn* __restrict__ qkv, T* __restrict__ q_out, FourBit
     const TIn* from = qkv + static_cast<long>(from_row) * s.row_width + static_cast<long>(head) * s.dim;
     if (head < s.q_heads) {
         float x[8];
-        make_eight<kSpan, TIn, float>(from, at, s, q_gain, pos, x);
+        make_eight<kSpan, kTurn, TIn, float>(from, at, lane, s, q_gain, pos, x);
         if (!exists || at >= s.dim) return;
         T* to = q_out + (static_cast<long>(row) * s.q_heads + head) * s.dim + at;
         if constexpr (sizeof(T) == 4) {
@@ -196,11 +222,16 @@ four_bit_fill_kernel(const TIn* __restrict__ qkv, T* __restrict__ q_out, FourBit
     }
     const bool is_key = head < s.q_heads + s.kv_heads;
     const int kvh = head - s.q_heads - (is_key ? 0 : s.kv_heads);
+    // where the row goes is looked up while its numbers are made
+    const int entry = row_entry[from_row];
+    const bool placed = exists && at < s.dim && pos >= 0 && entry >= 0 && entry < s.entries;
+    const int block = pos / s.page_tokens, token = pos - block * s.page_tokens;
+    const int page = placed ? mapped_page(block_table + static_cast<long>(entry) * s.max_blocks, block, s.max_blocks, pools.pages) : -1;
     int power;
     unsigned codes;
     if (is_key) {
         double x[8];
-        make_eight<kSpan, TIn, double>(from, at, s, k_gain, pos, x);
+        make_eight<kSpan, kTurn, TIn, double>(from, at, lane, s, k_gain, pos, x);
         codes = eight_codes(x, power);
     } else if (s.planes == 1) {
         float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -211,11 +242,6 @@ four_bit_fill_kernel(const TIn* __restrict__ qkv, T* __restrict__ q_out, FourBit
         if (at < s.dim) load_eight<TIn, double>(from + at, s.planes, s.plane, x);
         codes = eight_codes(x, power);
     }
-    if (!exists || at >= s.dim || pos < 0) return;
-    const int entry = row_entry[row];
-    if (entry < 0 || entry >= s.entries) return;
-    const int block = pos / s.page_tokens, token = pos - block * s.page_tokens;
-    const int page = mapped_page(block_table + static_cast<long>(entry) * s.max_blocks, block, s.max_blocks, pools.pages);
     if (page < 0) return;                                         // the host reserves the pages before the launch
     const long place = static_cast<long>(page) * s.kv_heads + kvh;
     const long code_base = place * four_bit_codes(s.page_tokens, s.dim), power_base = place * four_bit_powers(s.page_tokens, s.dim);
@@ -260,19 +286,31 @@ four_bit_rows_kernel(FourBitPools pools, const int* __restrict__ positions, cons
     *reinterpret_cast<uint4*>(v_out + to) = v;
 }
 
+template <int kSpan, typename TIn, typename T>
+static void launch_fill_span(const void* qkv, void* q_out, const FourBitPools& pools, AnyVec q_gain, AnyVec k_gain, const int* positions,
+                             const int* row_entry, const int* block_table, const FillShape& s, int turn, hipStream_t stream) {
+    const long waves = static_cast<long>(ceil_div(s.rows, kWave / kSpan)) * (s.q_heads + 2 * s.kv_heads);
+    const int blocks = ceil_div(waves, kFillThreads / kWave);
+#define LEONE_FILL(TURN)                                                                                                                  \
+    case TURN:                                                                                                                            \
+        four_bit_fill_kernel<kSpan, TURN, TIn, T><<<blocks, kFillThreads, 0, stream>>>(                                                   \
+            static_cast<const TIn*>(qkv), static_cast<T*>(q_out), pools, q_gain, k_gain, positions, row_entry, block_table, s);           \
+        break;
+    switch (turn) { LEONE_FILL(kNoTurn) LEONE_FILL(kWholeHalves) LEONE_FILL(kAnyTurn) }
+#undef LEONE_FILL
+}
+
 template <typename TIn, typename T>
 static void launch_fill(const void* qkv, void* q_out, const FourBitPools& pools, AnyVec q_gain, AnyVec k_gain, const int* positions,
                         const int* row_entry, const int* block_table, const FillShape& s, hipStream_t stream) {
     const int span = s.dim <= 32 ? 4 : s.dim <= 64 ? 8 : s.dim <= 128 ? 16 : 32;
-    const long waves = static_cast<long>(ceil_div(s.rows, kWave / span)) * (s.q_heads + 2 * s.kv_heads);
-    const int blocks = ceil_div(waves, kFillThreads / kWave);
-#define LEONE_FILL(SPAN)                                                                                                                    \
-    case SPAN:                                                                                                                              \
-        four_bit_fill_kernel<SPAN, TIn, T><<<blocks, kFillThreads, 0, stream>>>(static_cast<const TIn*>(qkv), static_cast<T*>(q_out), pools, \
-                                                                               q_gain, k_gain, positions, row_entry, block_table, s);      \
-        break;
-    switch (span) { LEONE_FILL(4) LEONE_FILL(8) LEONE_FILL(16) LEONE_FILL(32) }
-#undef LEONE_FILL
+    const bool aligned = (reinterpret_cast<uintptr_t>(s.cos_table) | reinterpret_cast<uintptr_t>(s.sin_table)) % 16 == 0;
+    const int turn = s.cos_table == nullptr ? kNoTurn
+                     : s.pairing == 0 && 2 * s.rotary_half == s.dim && s.dim == 8 * span && aligned ? kWholeHalves : kAnyTurn;
+#define LEONE_SPAN(SPAN)                                                                                                                       \
+    case SPAN: launch_fill_span<SPAN, TIn, T>(qkv, q_out, pools, q_gain, k_gain, positions, row_entry, block_table, s, turn, stream); break;
+    switch (span) { LEONE_SPAN(4) LEONE_SPAN(8) LEONE_SPAN(16) LEONE_SPAN(32) }
+#undef LEONE_SPAN
 }
 
 }  // namespace leone
