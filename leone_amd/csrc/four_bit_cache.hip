@@ -22,6 +22,7 @@ constexpr int kFillThreads = 256;
 
 struct FillShape {
     int rows, q_heads, kv_heads, dim, page_tokens, max_blocks, entries;
+    int page_shift;              // of pages of a power of two tokens, else -1
     long row_width;              // elements from row to row
     int planes;
     long plane;
@@ -31,20 +32,50 @@ struct FillShape {
     int table_positions, rotary_half, pairing;
 };
 
-// Eight neighbouring elements of a row, the planes of a product cut along K added up in order.
-template <typename TIn, typename Acc>
-__device__ inline void load_eight(const TIn* __restrict__ from, int planes, long plane, Acc out[8]) {
-    float part[8];
-    constexpr int code = sizeof(TIn) == 4 ? kF32 : kBF16;
-    load_any8(AnyVec{from, code}, 0, part);
+// Eight neighbouring elements as they were loaded, unpacked where they are used: what a row starts from is asked for at once, and
+// nothing waits for one before the next is asked for.
+template <typename TIn>
+struct Raw {
+    uint4 v[sizeof(TIn) / 2];
+    __device__ void load(const TIn* from) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = static_cast<Acc>(part[i]);
-    for (int s = 1; s < planes; ++s) {
-        load_any8(AnyVec{from, code}, s * plane, part);
+        for (unsigned i = 0; i < sizeof(TIn) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(from)[i];
+    }
+    template <typename Acc>
+    __device__ void get(Acc x[8]) const {
+        const unsigned w[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+        if constexpr (sizeof(TIn) == 4) {
+            const unsigned u[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(w[i]), x[4 + i] = __uint_as_float(u[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
+// The planes of a product cut along K added up in order, the first of them as it was loaded.
+template <typename TIn, typename Acc>
+__device__ inline void add_planes(const Raw<TIn>& first, const TIn* __restrict__ from, int planes, long plane, Acc out[8]) {
+    first.get(out);
+    for (int p = 1; p < planes; ++p) {
+        Raw<TIn> next;
+        float part[8];
+        next.load(from + p * plane);
+        next.get(part);
 #pragma unroll
         for (int i = 0; i < 8; ++i) out[i] += static_cast<Acc>(part[i]);
     }
 }
+// What a lane starts from beside its own elements: its gains, and (kWholeHalves) its angles.
+struct Beside {
+    uint4 gain[2];
+    float4 cosine[2], sine[2];
+    __device__ void gains(int dtype, float g[8]) const {
+        if (dtype == kF32) Raw<float>{{gain[0], gain[1]}}.get(g);
+        else Raw<bf16_t>{{gain[0]}}.get(g);
+    }
+};
 
 __device__ inline float root(float v) { return sqrtf(v); }
 __device__ inline double root(double v) { return sqrt(v); }
@@ -64,19 +95,14 @@ enum Turn : int { kNoTurn = 0, kWholeHalves = 1, kAnyTurn = 2 };
 // Eight elements of a query or key head: normed and rotated.  `at` is the lane's first element; lanes behind the head (at >= dim)
 // take part in the sum with nothing.
 template <int kSpan, int kTurn, typename TIn, typename Acc>
-__device__ inline void make_eight(const TIn* __restrict__ head, int at, int lane, const FillShape& s, const AnyVec& gain, int pos, Acc x[8]) {
+__device__ inline void make_eight(const Raw<TIn>& raw, const Beside& beside, const TIn* __restrict__ head, int at, int lane, const FillShape& s,
+                                  const AnyVec& gain, int pos, Acc x[8]) {
     const bool in_head = at < s.dim;
     const int half = s.rotary_half;
-    const long angles = static_cast<long>(pos < s.table_positions ? pos : s.table_positions - 1) * half;   // (the host checks the bound)
+    const long angles = static_cast<long>(max(pos < s.table_positions ? pos : s.table_positions - 1, 0)) * half;   // (the host checks the bound)
+    add_planes<TIn, Acc>(raw, head + at, in_head ? s.planes : 1, s.plane, x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0;
-    if (in_head) load_eight<TIn, Acc>(head + at, s.planes, s.plane, x);
-    float g[8], c[8], n[8];
-    if (gain.ptr && in_head) load_any8(gain, at, g);
-    if constexpr (kTurn == kWholeHalves) {
-        load_any8(AnyVec{s.cos_table, kF32}, angles + (at & (half - 1)), c);
-        load_any8(AnyVec{s.sin_table, kF32}, angles + (at & (half - 1)), n);
-    }
+    for (int i = 0; i < 8; ++i) x[i] = in_head ? x[i] : 0;
     // the partners, where they are not among the lane's own
     const bool turned = kTurn == kAnyTurn && at < 2 * half;
     const bool apart = turned && s.pairing == 0;
@@ -87,7 +113,9 @@ __device__ inline void make_eight(const TIn* __restrict__ head, int at, int lane
         for (int i = 0; i < 8; ++i) other[i] = 0;
         if (apart && in_head) {
             if (half % 8 == 0) {
-                load_eight<TIn, Acc>(head + partner(at), s.planes, s.plane, other);
+                Raw<TIn> theirs;
+                theirs.load(head + partner(at));
+                add_planes<TIn, Acc>(theirs, head + partner(at), s.planes, s.plane, other);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -105,9 +133,11 @@ __device__ inline void make_eight(const TIn* __restrict__ head, int at, int lane
         for (int i = 0; i < 8; ++i) squares += x[i] * x[i];
         squares = join_span<kSpan>(squares, [](Acc a, Acc b) { return a + b; });
         const Acc inv = Acc(1) / root(squares / static_cast<Acc>(s.dim) + static_cast<Acc>(s.eps));
-        if (in_head) {
+        float g[8];
+        beside.gains(gain.dtype, g);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * static_cast<Acc>(g[i]) * inv;
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * static_cast<Acc>(g[i]) * inv;
+        if (in_head) {
             if (apart) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -117,6 +147,10 @@ __device__ inline void make_eight(const TIn* __restrict__ head, int at, int lane
     }
     if constexpr (kTurn == kWholeHalves) {
         const bool first = (lane & (kSpan / 2)) == 0;
+        const float c[8] = {beside.cosine[0].x, beside.cosine[0].y, beside.cosine[0].z, beside.cosine[0].w,
+                            beside.cosine[1].x, beside.cosine[1].y, beside.cosine[1].z, beside.cosine[1].w};
+        const float n[8] = {beside.sine[0].x, beside.sine[0].y, beside.sine[0].z, beside.sine[0].w,
+                            beside.sine[1].x, beside.sine[1].y, beside.sine[1].z, beside.sine[1].w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const Acc o = of_partner<kSpan / 2>(x[i], lane), cosine = c[i], sine = first ? -n[i] : n[i];
@@ -194,19 +228,40 @@ four_bit_fill_kernel(const TIn* __restrict__ qkv, T* __restrict__ q_out, FourBit
                      const int* __restrict__ positions, const int* __restrict__ row_entry, const int* __restrict__ block_table, FillShape s) {
     constexpr int kRows = kWave / kSpan;                          // rows of one head a wave takes
     const int lane = threadIdx.x % kWave;
-    const int heads = s.q_heads + 2 * s.kv_heads;
-    const long item = static_cast<long>(blockIdx.x) * (kFillThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int row_run = static_cast<int>(item / heads), head = static_cast<int>(item - static_cast<long>(row_run) * heads);
-    if (row_run * kRows >= s.rows) return;
+    const int head = blockIdx.x * (kFillThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int row_run = blockIdx.y;
+    if (head >= s.q_heads + 2 * s.kv_heads) return;
     const int row = row_run * kRows + lane / kSpan;
     const int at = lane % kSpan * 8;
     const bool exists = row < s.rows;
     const int from_row = exists ? row : s.rows - 1;               // (every lane takes part in the exchanges)
-    const int pos = positions[from_row];
+    const bool is_query = head < s.q_heads, is_key = !is_query && head < s.q_heads + s.kv_heads;
     const TIn* from = qkv + static_cast<long>(from_row) * s.row_width + static_cast<long>(head) * s.dim;
-    if (head < s.q_heads) {
+    const int pos = positions[from_row], entry = row_entry[from_row];
+    const int read_at = min(at, s.dim - 8);                       // (lanes behind the head read its last eight and drop them)
+    Raw<TIn> raw;
+    raw.load(from + read_at);
+    const AnyVec gain = is_query ? q_gain : k_gain;
+    Beside beside;
+    if (gain.ptr != nullptr && (is_query || is_key)) {
+        if (gain.dtype == kF32) {
+            const uint4* g = reinterpret_cast<const uint4*>(static_cast<const float*>(gain.ptr) + read_at);
+            beside.gain[0] = g[0], beside.gain[1] = g[1];
+        } else {
+            beside.gain[0] = *reinterpret_cast<const uint4*>(static_cast<const bf16_t*>(gain.ptr) + read_at);
+        }
+    }
+    if constexpr (kTurn == kWholeHalves) {
+        if (is_query || is_key) {
+            const long angles = static_cast<long>(max(pos < s.table_positions ? pos : s.table_positions - 1, 0)) * s.rotary_half + (at & (s.rotary_half - 1));
+            const float4* c = reinterpret_cast<const float4*>(s.cos_table + angles);
+            const float4* n = reinterpret_cast<const float4*>(s.sin_table + angles);
+            beside.cosine[0] = c[0], beside.cosine[1] = c[1], beside.sine[0] = n[0], beside.sine[1] = n[1];
+        }
+    }
+    if (is_query) {
         float x[8];
-        make_eight<kSpan, kTurn, TIn, float>(from, at, lane, s, q_gain, pos, x);
+        make_eight<kSpan, kTurn, TIn, float>(raw, beside, from, at, lane, s, q_gain, pos, x);
         if (!exists || at >= s.dim) return;
         T* to = q_out + (static_cast<long>(row) * s.q_heads + head) * s.dim + at;
         if constexpr (sizeof(T) == 4) {
@@ -220,26 +275,24 @@ four_bit_fill_kernel(const TIn* __restrict__ qkv, T* __restrict__ q_out, FourBit
         }
         return;
     }
-    const bool is_key = head < s.q_heads + s.kv_heads;
     const int kvh = head - s.q_heads - (is_key ? 0 : s.kv_heads);
     // where the row goes is looked up while its numbers are made
-    const int entry = row_entry[from_row];
     const bool placed = exists && at < s.dim && pos >= 0 && entry >= 0 && entry < s.entries;
-    const int block = pos / s.page_tokens, token = pos - block * s.page_tokens;
+    const int block = s.page_shift >= 0 ? pos >> s.page_shift : pos / s.page_tokens, token = pos - block * s.page_tokens;
     const int page = placed ? mapped_page(block_table + static_cast<long>(entry) * s.max_blocks, block, s.max_blocks, pools.pages) : -1;
     int power;
     unsigned codes;
     if (is_key) {
         double x[8];
-        make_eight<kSpan, kTurn, TIn, double>(from, at, lane, s, k_gain, pos, x);
+        make_eight<kSpan, kTurn, TIn, double>(raw, beside, from, at, lane, s, k_gain, pos, x);
         codes = eight_codes(x, power);
     } else if (s.planes == 1) {
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (at < s.dim) load_eight<TIn, float>(from + at, 1, 0, x);
+        float x[8];
+        raw.get(x);
         codes = eight_codes(x, power);
     } else {
-        double x[8] = {0., 0., 0., 0., 0., 0., 0., 0.};
-        if (at < s.dim) load_eight<TIn, double>(from + at, s.planes, s.plane, x);
+        double x[8];
+        add_planes<TIn, double>(raw, from + read_at, s.planes, s.plane, x);
         codes = eight_codes(x, power);
     }
     if (page < 0) return;                                         // the host reserves the pages before the launch
@@ -289,8 +342,7 @@ four_bit_rows_kernel(FourBitPools pools, const int* __restrict__ positions, cons
 template <int kSpan, typename TIn, typename T>
 static void launch_fill_span(const void* qkv, void* q_out, const FourBitPools& pools, AnyVec q_gain, AnyVec k_gain, const int* positions,
                              const int* row_entry, const int* block_table, const FillShape& s, int turn, hipStream_t stream) {
-    const long waves = static_cast<long>(ceil_div(s.rows, kWave / kSpan)) * (s.q_heads + 2 * s.kv_heads);
-    const int blocks = ceil_div(waves, kFillThreads / kWave);
+    const dim3 blocks(ceil_div(s.q_heads + 2 * s.kv_heads, kFillThreads / kWave), ceil_div(s.rows, kWave / kSpan));
 #define LEONE_FILL(TURN)                                                                                                                  \
     case TURN:                                                                                                                            \
         four_bit_fill_kernel<kSpan, TURN, TIn, T><<<blocks, kFillThreads, 0, stream>>>(                                                   \
@@ -341,8 +393,9 @@ extern "C" int leone_four_bit_fill(const void* qkv, int qkv_dtype, int qkv_plane
     LEONE_REQUIRE(pairing == 0 || pairing == 1, "%s: unknown pairing %d", what, pairing);
     LEONE_REQUIRE((reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(q_gain) |
                    reinterpret_cast<uintptr_t>(k_gain)) % 16 == 0, "%s: the projection, the queries and the gains start at multiples of 16 bytes", what);
-    LEONE_REQUIRE(static_cast<long>(rows) * (q_heads + 2L * kv_heads) < 0x7fffffffL, "%s: too many rows for one launch", what);
-    const FillShape s{rows, q_heads, kv_heads, head_dim, page_tokens, max_blocks, entries, row_width, qkv_planes, qkv_plane, eps, cos_table,
+    LEONE_REQUIRE(rows <= 2 * 65535, "%s: too many rows for one launch", what);     // (two of 256 elements are the fewest a wave takes)
+    const int page_shift = (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1;
+    const FillShape s{rows, q_heads, kv_heads, head_dim, page_tokens, max_blocks, entries, page_shift, row_width, qkv_planes, qkv_plane, eps, cos_table,
                       sin_table, table_positions, cos_table ? rotary_dim / 2 : 0, pairing};
     const AnyVec qg{q_gain, gain_dtype}, kg{k_gain, gain_dtype};
     if (dtype == kF32) launch_fill<float, float>(qkv, q_out, pools, qg, kg, positions, row_entry, block_table, s, stream);
