@@ -55,7 +55,8 @@ struct PromptStage {
     uint4 values[8 * kD];                             // [run of eight tokens][place of the element]
 };
 
-template <int kD>
+// kWide: a stage's keys lie on one page, whose id is the same for the workgroup.
+template <int kD, bool kWide>
 __global__ void __launch_bounds__(kPromptThreads, 2)
 four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, FourBitPools pools, const int* __restrict__ positions,
                         const int* __restrict__ tiles, int n_groups, const int* __restrict__ block_table, int max_blocks, int entries,
@@ -70,6 +71,7 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
     __shared__ PromptStage<kD> stages[2];
     // Keys whose value block is NaN, of three stages in turn: one is read, one written and one cleared between two barriers.
     __shared__ unsigned long long nan_keys[3][kBlocks];
+    __shared__ int nan_seen[3];
     __shared__ int wave_lo[kPromptWaves], wave_hi[kPromptWaves];
     __shared__ int unmapped_seen;
 
@@ -93,6 +95,7 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
     }
     if (tid == 0) unmapped_seen = 0;
     if (tid < 3 * kBlocks) nan_keys[tid / kBlocks][tid % kBlocks] = 0;
+    if (tid < 3) nan_seen[tid] = 0;
     __syncthreads();
     int group_lo = 0x7fffffff, group_hi = 0;
 #pragma unroll
@@ -153,50 +156,65 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
         const int k_key = 32 * (tid / (32 * kBlocks)) + pass_key(tid & 31), k_block = tid / 32 % kBlocks;
         const int v_key = 4 * (tid / kEights), v_eight = tid % kEights;
         const int p_key = pass_key(j);
+        // The pages of a stage.  Loads are the same whatever the stage (what is behind the table reads its last place) and are not
+        // waited for before they are used, a stage later.
         struct Pages {
             int k, v, p[2];
         };
-        auto page_of = [&](int key) {
-            return key >= group_lo && key < group_hi ? mapped_page(table, key >> page_shift, max_blocks, pools.pages) : -1;
-        };
+        auto entry_of = [&](int key) { return table[min(key >> page_shift, max_blocks - 1)]; };
         auto find = [&](int t) {
             const int key0 = t * kStageKeys;
-            Pages at{-1, -1, {-1, -1}};
-            if (brings) {
-                at.k = page_of(key0 + k_key);
-                const int first = max(key0 + v_key, group_lo);                 // a run may begin before the first key in sight
-                at.v = first < key0 + v_key + 4 ? page_of(first) : -1;
+            Pages at;
+            if constexpr (kWide) {
+                at.k = at.v = at.p[0] = at.p[1] = entry_of(key0);
+            } else {
+                at.k = entry_of(key0 + k_key), at.v = entry_of(key0 + v_key);
+                at.p[0] = entry_of(key0 + p_key), at.p[1] = entry_of(key0 + 32 + p_key);
             }
-#pragma unroll
-            for (int half = 0; half < 2; ++half) at.p[half] = page_of(key0 + 32 * half + p_key);
             return at;
         };
+        auto mapped = [&](int page, int key) { return static_cast<unsigned>(page) < static_cast<unsigned>(pools.pages) && key >> page_shift < max_blocks; };
+        const unsigned code_stride = static_cast<unsigned>(code_bytes) * kv_heads, power_stride = static_cast<unsigned>(power_bytes) * kv_heads;
+        const uint8_t* k_codes_base = pools.k_codes + kvh * code_bytes;
+        const uint8_t* k_powers_base = pools.k_powers + kvh * power_bytes;
+        const uint8_t* v_codes_base = pools.v_codes + kvh * code_bytes;
+        const uint8_t* v_powers_base = pools.v_powers + kvh * power_bytes;
+        // a lane's own offsets from where the stage's first key, or (pages shorter than a stage) its own key's page begins
+        const unsigned k_code_at = four_bit_key(kWide ? k_key : k_key & page_mask, k_block, page_tokens);
+        const unsigned v_code_at = four_bit_value(kWide ? v_key : v_key & page_mask, v_eight, kD);
+        const unsigned v_power_at = four_bit_value_power(kWide ? v_key : v_key & page_mask, v_eight / 4, kD);
+        unsigned k_power_at[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) k_power_at[half] = four_bit_key_power(kWide ? 32 * half + p_key : (32 * half + p_key) & page_mask, 0, kD);
         uint4 v_codes = {0u, 0u, 0u, 0u};
         unsigned v_powers = 0x7f7f7f7fu;
         unsigned k_powers[2], k_powers_next[2];
         auto fetch = [&](int t, const Pages& at, PromptStage<kD>* to) {
             const int key0 = t * kStageKeys;
+            const unsigned token0 = kWide ? key0 & page_mask : 0;            // (pages shorter than a stage: it begins where one does)
+            auto place = [&](int page, int key, unsigned stride) {
+                return static_cast<unsigned long long>(mapped(page, key) ? page : 0) * stride;
+            };
+            // of a stage that is not wholly in sight, or has keys without a page, what is not there may be anything: a power of one
+            // makes it a number (its keys' scores are masked later)
+            const bool whole = key0 >= group_lo && key0 + kStageKeys <= group_hi;
             if (brings) {
-                const long place = static_cast<long>(max(at.k, 0)) * kv_heads + kvh;
-                const uint8_t* from = pools.k_codes + place * code_bytes + four_bit_key((key0 + k_key) & page_mask, k_block, page_tokens);
-                load_to_shared(from, to->keys + wave * kWave);
-                const long v_place = static_cast<long>(max(at.v, 0)) * kv_heads + kvh;
-                const int token = (key0 + v_key) & page_mask;
-                v_codes = *reinterpret_cast<const uint4*>(pools.v_codes + v_place * code_bytes + four_bit_value(token, v_eight, kD));
-                v_powers = *reinterpret_cast<const unsigned*>(pools.v_powers + v_place * power_bytes + four_bit_value_power(token, v_eight / 4, kD));
-                if ((key0 + k_key >= group_lo && key0 + k_key < group_hi && at.k < 0)) unmapped_seen = 1;
-                if (key0 + v_key < group_lo || key0 + v_key + 4 > group_hi || at.v < 0) {      // out of sight: may be anything
+                const int key = key0 + (kWide ? 0 : k_key), v_first = key0 + (kWide ? 0 : v_key);
+                load_to_shared(k_codes_base + place(at.k, key, code_stride) + 16 * token0 + k_code_at, to->keys + wave * kWave);
+                v_codes = *reinterpret_cast<const uint4*>(v_codes_base + place(at.v, v_first, code_stride) + kD / 2 * token0 + v_code_at);
+                v_powers = *reinterpret_cast<const unsigned*>(v_powers_base + place(at.v, v_first, power_stride) + kBlocks * token0 + v_power_at);
+                if (!mapped(at.k, key) && key0 + k_key >= group_lo && key0 + k_key < group_hi) unmapped_seen = 1;
+                if (!whole || !mapped(at.v, v_first)) {
                     unsigned hidden = 0;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (key0 + v_key + i < group_lo || key0 + v_key + i >= group_hi || at.v < 0) hidden |= 0xffu << (8 * i);
+                        if (key0 + v_key + i < group_lo || key0 + v_key + i >= group_hi || !mapped(at.v, v_first)) hidden |= 0xffu << (8 * i);
                     v_powers = (v_powers & ~hidden) | (0x7f7f7f7fu & hidden);
                 }
             }
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const long place = static_cast<long>(max(at.p[half], 0)) * kv_heads + kvh;
-                const uint8_t* from = pools.k_powers + place * power_bytes + four_bit_key_power((key0 + 32 * half + p_key) & page_mask, 0, kD);
+                const uint8_t* from = k_powers_base + place(at.p[half], key0 + (kWide ? 0 : 32 * half + p_key), power_stride) + kBlocks * token0 + k_power_at[half];
                 if constexpr (kBlocks == 4) k_powers_next[half] = *reinterpret_cast<const unsigned*>(from);
                 else k_powers_next[half] = *reinterpret_cast<const unsigned short*>(from);
             }
@@ -213,6 +231,7 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (nan_tokens >> i & 1u) words[i] = 0, powers = (powers & ~(0xffu << (8 * i))) | (0x7fu << (8 * i));
+                    nan_seen[t % 3] = 1;
                     atomicOr(&nan_keys[t % 3][v_eight / 4], static_cast<unsigned long long>(nan_tokens) << v_key);
                 }
                 float power[4];
@@ -299,6 +318,7 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
             return (at % kEights) / 4;
         };
         auto spoil = [&](int t) {
+            if (nan_seen[t % 3] == 0) return;
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
                 const unsigned long long keys = nan_keys[t % 3][b];
@@ -337,6 +357,7 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
             }
             spoil(t);
             if (tid < kBlocks) nan_keys[(t + 2) % 3][tid] = 0;
+            if (tid == 0) nan_seen[(t + 2) % 3] = 0;
             if (more) {
                 deposit(t + 1, writing);
                 k_powers[0] = k_powers_next[0], k_powers[1] = k_powers_next[1];
@@ -413,16 +434,23 @@ extern "C" int leone_four_bit_prefill(const void* q, void* out, const void* k_co
                   kMaxRanges);
     LEONE_REQUIRE(splits == 1 || (part_acc && part_ml && reinterpret_cast<uintptr_t>(part_acc) % 16 == 0), "%s: %d ranges need the workspace", what, splits);
     LEONE_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 == 0, "%s: queries and results start at multiples of 16 bytes", what);
+    LEONE_REQUIRE(four_bit_codes(page_tokens, head_dim) * kv_heads < 0x7fffffffL, "%s: a page of %d heads is too large", what, kv_heads);
     int page_shift = 0;
     while ((1 << page_shift) < page_tokens) ++page_shift;
     const dim3 grid(n_groups * q_heads, splits);
-#define LEONE_PREFILL(D)                                                                                                                       \
-    four_bit_prefill_kernel<D><<<grid, kPromptThreads, 0, stream>>>(static_cast<const bf16_t*>(q), static_cast<bf16_t*>(out), pools, positions, \
-                                                                    tiles, n_groups, block_table, max_blocks, entries, q_heads, kv_heads,      \
-                                                                    page_shift, scale * kLog2e, window, splits, part_acc, part_ml)
+#define LEONE_PREFILL_CALL(D, WIDE)                                                                                                            \
+    four_bit_prefill_kernel<D, WIDE><<<grid, kPromptThreads, 0, stream>>>(static_cast<const bf16_t*>(q), static_cast<bf16_t*>(out), pools,     \
+                                                                          positions, tiles, n_groups, block_table, max_blocks, entries, q_heads, \
+                                                                          kv_heads, page_shift, scale * kLog2e, window, splits, part_acc, part_ml)
+#define LEONE_PREFILL(D)                                             \
+    do {                                                             \
+        if (page_tokens >= kStageKeys) LEONE_PREFILL_CALL(D, true);  \
+        else LEONE_PREFILL_CALL(D, false);                           \
+    } while (0)
     if (head_dim == 64) LEONE_PREFILL(64);
     else LEONE_PREFILL(128);
 #undef LEONE_PREFILL
+#undef LEONE_PREFILL_CALL
     LEONE_LAUNCH_CHECK(what);
     if (splits > 1) {
         merge_four_bit_shares(part_acc, part_ml, out, kBF16, static_cast<long>(n_groups) * kPromptWaves * kTileRows, q_heads, head_dim, splits, tiles, stream);
