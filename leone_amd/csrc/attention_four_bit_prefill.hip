@@ -2,11 +2,12 @@
 // 128.
 //
 // A wave takes a tile of 32 consecutive rows of one request and one query head, a workgroup four tiles of the request (the host lists
-// them: entry, first row, rows); it walks the keys its tiles can see once, 64 at a time.  Keys go from the cache to shared memory as
-// they are, by loads that write there themselves, and into the first product as they are:
+// them: entry, first row, rows); it walks the keys its tiles can see once, 64 at a time.  Keys go from the cache to shared memory and
+// into the first product as they are:
 // v_mfma_scale_f32_32x32x64_f8f6f4, 4-bit keys with their powers against queries in two 8-bit parts (see attention_four_bit.hip).  It takes as
 // long as the bfloat16 product of the same size would, but a wave reads a quarter of the bytes from shared memory, which four waves
-// with 32 rows each read all keys from.  Values are unpacked once for the four waves: a thread has four tokens of eight elements
+// with 32 rows each read all keys from.  (By loads that write to shared memory themselves the compiler waits for the next stage's
+// before it reads this one's: 322 us where this takes 2xx.)  Values are unpacked once for the four waves: a thread has four tokens of eight elements
 // in flight while a stage is worked on, turns them into runs of eight tokens of one element and leaves them in shared memory for
 // the next, in bfloat16, where v_mfma_f32_32x32x16_bf16 takes them.
 //
@@ -40,14 +41,10 @@ constexpr int kPromptThreads = kPromptWaves * kWave;
 constexpr int kStageKeys = 64;
 constexpr int kPassKeys = 32;
 constexpr int kMaxRanges = 32;
+constexpr int kPromptUnits = 256;                     // compute units: workgroups that get one of their own
 
 // Row of a pass's first product <-> key of the pass.
 __device__ inline int pass_key(int x) { return (x & 0x13) | ((x & 4) << 1) | ((x & 8) >> 1); }
-
-// Sixteen bytes a lane straight into shared memory, the lanes' one after the other from `to` (the same for the wave).
-__device__ inline void load_to_shared(const uint8_t* from, uint4* to) {
-    __builtin_amdgcn_global_load_lds(reinterpret_cast<const uint4*>(from), to, 16, 0, 0);
-}
 
 template <int kD>
 struct PromptStage {
@@ -77,6 +74,9 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
     const int j = lane & 31, h = lane >> 5;
+    // Two workgroups share a unit: the second half of those that fit at a time goes first where both have something to issue, so that one
+    // multiplies while the other makes weights instead of both doing the same (2,048 rows behind 8,192 tokens 322 us without, 308 with).
+    if ((blockIdx.x + blockIdx.y * gridDim.x) / kPromptUnits % 2) __builtin_amdgcn_s_setprio(1);
     const PrefillWork work = prefill_work(static_cast<int>(blockIdx.x), q_heads, n_groups);
     const int head = work.head, kvh = head / (q_heads / kv_heads);
     const int page_tokens = 1 << page_shift, page_mask = page_tokens - 1;
@@ -148,7 +148,7 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
             }
         }
 
-        // ---- bringing a stage: a thread's unit of keys is block `k_block` of key k_key, its values eight `v_eight` of the four tokens
+        // ---- bringing a stage by way of registers, a stage ahead: a thread's unit of keys is block `k_block` of key k_key, its values eight `v_eight` of the four tokens
         // from v_key; a wave's lanes also hold the powers of the keys that they multiply.
         const int* table = block_table + static_cast<long>(entry) * max_blocks;
         const long code_bytes = four_bit_codes(page_tokens, kD), power_bytes = four_bit_powers(page_tokens, kD);
@@ -174,7 +174,8 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
             return at;
         };
         auto mapped = [&](int page, int key) { return static_cast<unsigned>(page) < static_cast<unsigned>(pools.pages) && key >> page_shift < max_blocks; };
-        const unsigned code_stride = static_cast<unsigned>(code_bytes) * kv_heads, power_stride = static_cast<unsigned>(power_bytes) * kv_heads;
+        // (a page's powers are a sixteenth of its codes)
+        const unsigned code_stride = static_cast<unsigned>(code_bytes) * kv_heads;
         const uint8_t* k_codes_base = pools.k_codes + kvh * code_bytes;
         const uint8_t* k_powers_base = pools.k_powers + kvh * power_bytes;
         const uint8_t* v_codes_base = pools.v_codes + kvh * code_bytes;
@@ -186,35 +187,34 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
         unsigned k_power_at[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) k_power_at[half] = four_bit_key_power(kWide ? 32 * half + p_key : (32 * half + p_key) & page_mask, 0, kD);
-        uint4 v_codes = {0u, 0u, 0u, 0u};
+        uint4 k_codes = {0u, 0u, 0u, 0u}, v_codes = {0u, 0u, 0u, 0u};
         unsigned v_powers = 0x7f7f7f7fu;
         unsigned k_powers[2], k_powers_next[2];
-        auto fetch = [&](int t, const Pages& at, PromptStage<kD>* to) {
+        auto fetch = [&](int t, const Pages& at) {
             const int key0 = t * kStageKeys;
             const unsigned token0 = kWide ? key0 & page_mask : 0;            // (pages shorter than a stage: it begins where one does)
-            auto place = [&](int page, int key, unsigned stride) {
-                return static_cast<unsigned long long>(mapped(page, key) ? page : 0) * stride;
-            };
+            auto place = [&](int page, int key) { return static_cast<unsigned long long>(mapped(page, key) ? page : 0) * code_stride; };
             // of a stage that is not wholly in sight, or has keys without a page, what is not there may be anything: a power of one
             // makes it a number (its keys' scores are masked later)
-            const bool whole = key0 >= group_lo && key0 + kStageKeys <= group_hi;
             if (brings) {
                 const int key = key0 + (kWide ? 0 : k_key), v_first = key0 + (kWide ? 0 : v_key);
-                load_to_shared(k_codes_base + place(at.k, key, code_stride) + 16 * token0 + k_code_at, to->keys + wave * kWave);
-                v_codes = *reinterpret_cast<const uint4*>(v_codes_base + place(at.v, v_first, code_stride) + kD / 2 * token0 + v_code_at);
-                v_powers = *reinterpret_cast<const unsigned*>(v_powers_base + place(at.v, v_first, power_stride) + kBlocks * token0 + v_power_at);
-                if (!mapped(at.k, key) && key0 + k_key >= group_lo && key0 + k_key < group_hi) unmapped_seen = 1;
-                if (!whole || !mapped(at.v, v_first)) {
+                const unsigned long long k_place = place(at.k, key), v_place = kWide ? k_place : place(at.v, v_first);
+                k_codes = *reinterpret_cast<const uint4*>(k_codes_base + (k_place + 16 * token0) + k_code_at);
+                v_codes = *reinterpret_cast<const uint4*>(v_codes_base + (v_place + kD / 2 * token0) + v_code_at);
+                v_powers = *reinterpret_cast<const unsigned*>(v_powers_base + (v_place / 16 + kBlocks * token0) + v_power_at);
+                const bool k_mapped = mapped(at.k, key), v_mapped = mapped(at.v, v_first);
+                if (key0 < group_lo || key0 + kStageKeys > group_hi || !k_mapped || !v_mapped) {
+                    if (!k_mapped && key0 + k_key >= group_lo && key0 + k_key < group_hi) unmapped_seen = 1;
                     unsigned hidden = 0;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (key0 + v_key + i < group_lo || key0 + v_key + i >= group_hi || !mapped(at.v, v_first)) hidden |= 0xffu << (8 * i);
+                        if (key0 + v_key + i < group_lo || key0 + v_key + i >= group_hi || !v_mapped) hidden |= 0xffu << (8 * i);
                     v_powers = (v_powers & ~hidden) | (0x7f7f7f7fu & hidden);
                 }
             }
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const uint8_t* from = k_powers_base + place(at.p[half], key0 + (kWide ? 0 : 32 * half + p_key), power_stride) + kBlocks * token0 + k_power_at[half];
+                const uint8_t* from = k_powers_base + (place(at.p[half], key0 + (kWide ? 0 : 32 * half + p_key)) / 16 + kBlocks * token0) + k_power_at[half];
                 if constexpr (kBlocks == 4) k_powers_next[half] = *reinterpret_cast<const unsigned*>(from);
                 else k_powers_next[half] = *reinterpret_cast<const unsigned short*>(from);
             }
@@ -222,6 +222,7 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
         // The values on their way into shared memory: by token, two elements at a time, then by element.
         auto deposit = [&](int t, PromptStage<kD>* to) {
             if (brings) {
+                to->keys[tid] = k_codes;
                 unsigned nan_tokens = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) nan_tokens |= (v_powers >> (8 * i) & 255u) == 255u ? 1u << i : 0u;
@@ -336,24 +337,24 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
         };
 
         const int t_begin = group_lo / kStageKeys, t_end = (group_hi + kStageKeys - 1) / kStageKeys;
-        auto arrived = [&]() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
-        fetch(t_begin, find(t_begin), &stages[0]);
+        // stages of which every row of the wave sees every key
+        const int plain_begin = (max(full_lo, group_lo) + kStageKeys - 1) / kStageKeys, plain_end = min(full_hi, group_hi) / kStageKeys;
+        fetch(t_begin, find(t_begin));
         Pages ahead = find(t_begin + 1);
-        arrived();
         deposit(t_begin, &stages[0]);
         k_powers[0] = k_powers_next[0], k_powers[1] = k_powers_next[1];
         __syncthreads();
         auto round = [&](const PromptStage<kD>* __restrict__ reading, PromptStage<kD>* __restrict__ writing, int t) {
             const bool more = t + 1 < t_end;
             if (more) {
-                fetch(t + 1, ahead, writing);
+                fetch(t + 1, ahead);
                 ahead = find(t + 2);
             }
+            const bool plain = t >= plain_begin && t < plain_end;    // nothing to mask: most stages of a long context
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int key0 = t * kStageKeys + half * kPassKeys;
-                if (key0 >= key_hi || key0 + kPassKeys <= key_lo) continue;
-                pass(reading, key0, half, key0 >= full_lo && key0 + kPassKeys <= full_hi && key0 >= group_lo && key0 + kPassKeys <= group_hi);
+                if (plain || (key0 < key_hi && key0 + kPassKeys > key_lo)) pass(reading, key0, half, plain);
             }
             spoil(t);
             if (tid < kBlocks) nan_keys[(t + 2) % 3][tid] = 0;
@@ -366,7 +367,6 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
         for (int t = t_begin; t < t_end; ++t) {
             const int cur = (t - t_begin) & 1;
             round(&stages[cur], &stages[cur ^ 1], t);
-            arrived();
             __syncthreads();
         }
     }
@@ -377,39 +377,33 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
     if (poisoned && row_pos >= 0) l_row = __builtin_nanf("");
     if (l_row != l_row) m_ref = fmaxf(m_ref, 0.f);               // (a result of NaN counts, whatever its maximum)
     const bool nothing = m_ref == -INFINITY;
+    const long row_head = static_cast<long>(tile_row0 + j) * q_heads + head, slot = row_head * splits + blockIdx.y;
     if (splits > 1) {
-        const long slot = (static_cast<long>(tile_row0 + j) * q_heads + head) * splits + blockIdx.y;
         if (h == 0) part_ml[2 * slot] = m_ref, part_ml[2 * slot + 1] = l_row;
         if (nothing) return;
-        float* to = part_acc + slot * kD;
-#pragma unroll
-        for (int dt = 0; dt < kDT; ++dt)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int at = 32 * dt + 8 * (v / 4) + 4 * h + v % 4;
-                to[8 * (at % kEights) + at / kEights] = acc[dt][v];
-            }
-        return;
     }
     const float inv = nothing ? 0.f : 1.f / l_row;
-    bf16_t* to = out + (static_cast<long>(tile_row0 + j) * q_heads + head) * kD;
-    // Places that differ by a whole row of eights are neighbouring elements: registers of the same place % kEights, in the order of the places.
-    constexpr int kMine = kEights / 2;                            // eights a lane has
+    // Places that differ by a whole row of eights are neighbouring elements: registers of the same place % kEights, in the order of the
+    // places, are the eight elements of one eight.
 #pragma unroll
-    for (int e = 0; e < kMine; ++e) {
+    for (int e = 0; e < kEights / 2; ++e) {
         const int at0 = 8 * (e / 4) + e % 4;                      // its place, 4 h aside
-        unsigned w[4];
+        float x[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            unsigned two[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int at = at0 + (2 * i + k) * kEights, dt = at / 32, r = at % 32;
-                two[k] = bf16_bits_from_float(acc[dt][4 * (r / 8) + r % 4] * inv);
-            }
-            w[i] = two[0] | two[1] << 16;
+        for (int i = 0; i < 8; ++i) {
+            const int at = at0 + i * kEights, dt = at / 32, r = at % 32;
+            x[i] = acc[dt][4 * (r / 8) + r % 4];
         }
-        *reinterpret_cast<uint4*>(to + 8 * (at0 + 4 * h)) = uint4{w[0], w[1], w[2], w[3]};
+        if (splits > 1) {
+            floatx4* to = reinterpret_cast<floatx4*>(part_acc + slot * kD + 8 * (at0 + 4 * h));
+            to[0] = floatx4{x[0], x[1], x[2], x[3]}, to[1] = floatx4{x[4], x[5], x[6], x[7]};
+        } else {
+            unsigned w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                w[i] = bf16_bits_from_float(x[2 * i] * inv) | static_cast<unsigned>(bf16_bits_from_float(x[2 * i + 1] * inv)) << 16;
+            *reinterpret_cast<uint4*>(out + row_head * kD + 8 * (at0 + 4 * h)) = uint4{w[0], w[1], w[2], w[3]};
+        }
     }
 }
 
