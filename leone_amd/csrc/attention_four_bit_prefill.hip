@@ -339,34 +339,38 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
         const int t_begin = group_lo / kStageKeys, t_end = (group_hi + kStageKeys - 1) / kStageKeys;
         // stages of which every row of the wave sees every key
         const int plain_begin = (max(full_lo, group_lo) + kStageKeys - 1) / kStageKeys, plain_end = min(full_hi, group_hi) / kStageKeys;
+        // Stage t + 1 is brought to shared memory in the middle of round t, from registers that were asked for a round before: the
+        // instructions that unpack it go beside the first half's second product.  (Every round asks for a stage, the last one again
+        // where there is no further: see `find`.)
         fetch(t_begin, find(t_begin));
-        Pages ahead = find(t_begin + 1);
+        Pages ahead = find(min(t_begin + 1, t_end - 1));
         deposit(t_begin, &stages[0]);
+        unsigned k_powers_ready[2] = {k_powers_next[0], k_powers_next[1]};
         k_powers[0] = k_powers_next[0], k_powers[1] = k_powers_next[1];
+        fetch(min(t_begin + 1, t_end - 1), ahead);
+        ahead = find(min(t_begin + 2, t_end - 1));
         __syncthreads();
         auto round = [&](const PromptStage<kD>* __restrict__ reading, PromptStage<kD>* __restrict__ writing, int t) {
-            const bool more = t + 1 < t_end;
-            if (more) {
-                fetch(t + 1, ahead);
-                ahead = find(t + 2);
-            }
             const bool plain = t >= plain_begin && t < plain_end;    // nothing to mask: most stages of a long context
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int key0 = t * kStageKeys + half * kPassKeys;
                 if (plain || (key0 < key_hi && key0 + kPassKeys > key_lo)) pass(reading, key0, half, plain);
+                if (half == 0) {
+                    if (t + 1 < t_end) deposit(t + 1, writing);
+                    k_powers_ready[0] = k_powers_next[0], k_powers_ready[1] = k_powers_next[1];
+                    fetch(min(t + 2, t_end - 1), ahead);
+                    ahead = find(min(t + 3, t_end - 1));
+                }
             }
             spoil(t);
             if (tid < kBlocks) nan_keys[(t + 2) % 3][tid] = 0;
             if (tid == 0) nan_seen[(t + 2) % 3] = 0;
-            if (more) {
-                deposit(t + 1, writing);
-                k_powers[0] = k_powers_next[0], k_powers[1] = k_powers_next[1];
-            }
         };
         for (int t = t_begin; t < t_end; ++t) {
             const int cur = (t - t_begin) & 1;
             round(&stages[cur], &stages[cur ^ 1], t);
+            k_powers[0] = k_powers_ready[0], k_powers[1] = k_powers_ready[1];
             __syncthreads();
         }
     }
