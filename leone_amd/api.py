@@ -46,11 +46,12 @@ def sampling_params(temperature: Optional[float] = None, seed: int = 0, top_k: O
     return params
 
 
-def cache_bytes_per_token(model) -> int:
+def cache_bytes_per_token(model, cache_bits: Optional[int] = None) -> int:
     """Bytes one cached token takes over all cache slots of the model: every paged need says its own
-    (``bytes_per_token(element size)``), whatever kind of cache it is."""
+    (``bytes_per_token(element size)``), whatever kind of cache it is.  ``cache_bits``: as for the engine."""
     size = torch.empty((), dtype=model.dtype).element_size()
-    return sum(need.bytes_per_token(size) for need in model.cache_needs().values() if getattr(need, "paged", False))
+    needs = model.cache_needs() if cache_bits is None else model.cache_needs(cache_bits)
+    return sum(need.bytes_per_token(size) for need in needs.values() if getattr(need, "paged", False))
 
 
 def default_num_pages(model, page_tokens: int, max_requests: int, max_context: int, bytes_per_token: int) -> int:
@@ -66,8 +67,9 @@ class Runtime:
     def __init__(self, model, *, num_pages: Optional[int] = None, max_tokens: Optional[int] = None,
                  page_tokens: int = 64, max_requests: int = 64, max_context: Optional[int] = None,
                  policy: Optional[SchedulerPolicy] = None, tokenizer=None, graphs: bool = True,
-                 poison_freed: bool = False, streamed_weights: Optional[bool] = None, tune_products: bool = False):
-        """``tune_products``: let the vendor library's products of a full prompt portion (the policy's
+                 poison_freed: bool = False, streamed_weights: Optional[bool] = None, tune_products: bool = False,
+                 cache_bits: Optional[int] = None):
+        """``cache_bits`` 4: keys and values in 4 bits an element (``Engine``).  ``tune_products``: let the vendor library's products of a full prompt portion (the policy's
         ``prefill_chunk_tokens``) run with the fastest of the library's algorithms, measured now (a few
         seconds; ``Engine.tune_products``)."""
         self.model = model
@@ -75,10 +77,10 @@ class Runtime:
         self.config = getattr(model, "config", None)
         context = min(max_context or model.spec.max_positions, model.spec.max_positions)
         if num_pages is None and max_tokens is None:
-            num_pages = default_num_pages(model, page_tokens, max_requests, context, cache_bytes_per_token(model))
+            num_pages = default_num_pages(model, page_tokens, max_requests, context, cache_bytes_per_token(model, cache_bits))
         self.engine = Engine(model, num_pages=num_pages, max_tokens=max_tokens, page_tokens=page_tokens,
                              max_requests=max_requests, max_context=context, graphs=graphs,
-                             poison_freed=poison_freed, streamed_weights=streamed_weights)
+                             poison_freed=poison_freed, streamed_weights=streamed_weights, cache_bits=cache_bits)
         self.policy = policy or SchedulerPolicy(max_live_requests=max_requests)
         self.tuned_products = []
         if tune_products and model.dtype == torch.bfloat16:

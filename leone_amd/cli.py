@@ -90,6 +90,8 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--ignore-eos", action="store_true", help="Do not stop at the end token")
     g.add_argument("--single-weight-copy", action="store_true",
                    help="Keep no second copy of the matrices in the decode kernels' order (half the weight memory, slower decoding)")
+    g.add_argument("--cache-bits", type=int, choices=[4], default=None,
+                   help="Keep keys and values in 4 bits an element: 3.76 times the tokens in the memory of a bfloat16 cache (the model's type)")
     g.add_argument("--tune-products", action="store_true",
                    help="Time the vendor library's algorithms for a full prompt portion first and use the fastest (a few seconds)")
     _add_sampling(g)
@@ -108,6 +110,7 @@ def build_parser() -> argparse.ArgumentParser:
     e.add_argument("--position-limit", type=int, default=None, help="Stop after n positions")
     e.add_argument("--prefill-chunk", type=int, default=None, help="Cut every window into portions of n tokens")
     e.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    e.add_argument("--cache-bits", type=int, choices=[4], default=None, help="Keep keys and values in 4 bits an element (the model's type)")
 
     r = sub.add_parser("random-model", help="Write a model folder with seeded random weights")
     r.add_argument("--config", required=True, help="config.json to build from")
@@ -138,7 +141,7 @@ def cmd_generate(args) -> int:
     runtime = Runtime.load(args.model, args.dtype, max_requests=1, max_context=args.max_context,
                            graphs=not args.eager_decode,
                            streamed_weights=False if args.single_weight_copy else None,
-                           tune_products=args.tune_products,
+                           tune_products=args.tune_products, cache_bits=args.cache_bits,
                            policy=SchedulerPolicy(max_live_requests=1, prefill_chunk_tokens=args.prefill_chunk,
                                                   max_step_tokens=max(args.prefill_chunk, 1)))
     if args.prompt is not None:
@@ -305,7 +308,7 @@ def cmd_eval(args) -> int:
         raise SystemExit("error: --window must be at least 2")
     model = load_model(args.model, args.dtype)
     window = min(args.window, model.spec.max_positions)
-    engine = Engine(model, max_tokens=window + 64, page_tokens=64, max_requests=1, max_context=window)
+    engine = Engine(model, max_tokens=window + 64, page_tokens=64, max_requests=1, max_context=window, cache_bits=args.cache_bits)
     rows = 0
     digest = hashlib.sha256()
     with open(args.logits, "wb") as out:

@@ -23,6 +23,7 @@ constexpr int kFillThreads = 256;
 struct FillShape {
     int rows, q_heads, kv_heads, dim, page_tokens, max_blocks, entries;
     int page_shift;              // of pages of a power of two tokens, else -1
+    int kv_written;              // key and value heads that are written: all or none
     long row_width;              // elements from row to row
     int planes;
     long plane;
@@ -230,7 +231,7 @@ four_bit_fill_kernel(const TIn* __restrict__ qkv, T* __restrict__ q_out, FourBit
     const int lane = threadIdx.x % kWave;
     const int head = blockIdx.x * (kFillThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int row_run = blockIdx.y;
-    if (head >= s.q_heads + 2 * s.kv_heads) return;
+    if (head >= s.q_heads + s.kv_written) return;
     const int row = row_run * kRows + lane / kSpan;
     const int at = lane % kSpan * 8;
     const bool exists = row < s.rows;
@@ -342,7 +343,7 @@ four_bit_rows_kernel(FourBitPools pools, const int* __restrict__ positions, cons
 template <int kSpan, typename TIn, typename T>
 static void launch_fill_span(const void* qkv, void* q_out, const FourBitPools& pools, AnyVec q_gain, AnyVec k_gain, const int* positions,
                              const int* row_entry, const int* block_table, const FillShape& s, int turn, hipStream_t stream) {
-    const dim3 blocks(ceil_div(s.q_heads + 2 * s.kv_heads, kFillThreads / kWave), ceil_div(s.rows, kWave / kSpan));
+    const dim3 blocks(ceil_div(s.q_heads + s.kv_written, kFillThreads / kWave), ceil_div(s.rows, kWave / kSpan));
 #define LEONE_FILL(TURN)                                                                                                                  \
     case TURN:                                                                                                                            \
         four_bit_fill_kernel<kSpan, TURN, TIn, T><<<blocks, kFillThreads, 0, stream>>>(                                                   \
@@ -374,7 +375,7 @@ extern "C" int leone_four_bit_fill(const void* qkv, int qkv_dtype, int qkv_plane
                                    const void* k_gain, int gain_dtype, float eps, const float* cos_table, const float* sin_table,
                                    int table_positions, int rotary_dim, int pairing, const int* positions, const int* row_entry,
                                    const int* block_table, int max_blocks, int entries, int rows, int q_heads, int kv_heads, int head_dim,
-                                   int page_tokens, hipStream_t stream) {
+                                   int page_tokens, int write_cache, hipStream_t stream) {
     const char* what = "four_bit_fill";
     const FourBitPools pools{static_cast<uint8_t*>(k_codes), static_cast<uint8_t*>(k_powers), static_cast<uint8_t*>(v_codes),
                              static_cast<uint8_t*>(v_powers), pages};
@@ -395,7 +396,7 @@ extern "C" int leone_four_bit_fill(const void* qkv, int qkv_dtype, int qkv_plane
                    reinterpret_cast<uintptr_t>(k_gain)) % 16 == 0, "%s: the projection, the queries and the gains start at multiples of 16 bytes", what);
     LEONE_REQUIRE(rows <= 2 * 65535, "%s: too many rows for one launch", what);     // (two of 256 elements are the fewest a wave takes)
     const int page_shift = (page_tokens & (page_tokens - 1)) == 0 ? __builtin_ctz(page_tokens) : -1;
-    const FillShape s{rows, q_heads, kv_heads, head_dim, page_tokens, max_blocks, entries, page_shift, row_width, qkv_planes, qkv_plane, eps, cos_table,
+    const FillShape s{rows, q_heads, kv_heads, head_dim, page_tokens, max_blocks, entries, page_shift, write_cache ? 2 * kv_heads : 0, row_width, qkv_planes, qkv_plane, eps, cos_table,
                       sin_table, table_positions, cos_table ? rotary_dim / 2 : 0, pairing};
     const AnyVec qg{q_gain, gain_dtype}, kg{k_gain, gain_dtype};
     if (dtype == kF32) launch_fill<float, float>(qkv, q_out, pools, qg, kg, positions, row_entry, block_table, s, stream);

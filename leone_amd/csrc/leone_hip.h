@@ -565,13 +565,13 @@ int leone_state_slots(const void* table, int tensors, long chunks, int move, con
 // head_dim / 32, 4], bytes that start at multiples of 16.  head_dim a multiple of 32 up to 256, page_tokens one of 8 up to 4,096.
 // Block tables are [entries, max_blocks]; what names no page (below 0, or not below `pages`) is neither read nor written.
 //
-// leone_qk_norm_rope_write for such a cache: heads normed (gains may be null) and rotated (tables may be null), q to q_out, k and
+// leone_qk_norm_rope_write for such a cache (write_cache 0: the queries alone): heads normed (gains may be null) and rotated (tables may be null), q to q_out, k and
 // v into the cache.  Rows of row_width elements; the projection, q_out and the gains start at multiples of 16 bytes.
 int leone_four_bit_fill(const void* qkv, int qkv_dtype, int qkv_planes, long qkv_plane, long row_width, void* q_out, int dtype,
                         void* k_codes, void* k_powers, void* v_codes, void* v_powers, int pages, const void* q_gain, const void* k_gain,
                         int gain_dtype, float eps, const float* cos_table, const float* sin_table, int table_positions, int rotary_dim,
                         int pairing, const int* positions, const int* row_entry, const int* block_table, int max_blocks, int entries, int rows,
-                        int q_heads, int kv_heads, int head_dim, int page_tokens, hipStream_t stream);
+                        int q_heads, int kv_heads, int head_dim, int page_tokens, int write_cache, hipStream_t stream);
 
 // What the cache holds at the rows' positions, bfloat16 [rows, kv_heads * head_dim] each; NaN where there is no page.
 int leone_four_bit_rows(const void* k_codes, const void* k_powers, const void* v_codes, const void* v_powers, int pages,

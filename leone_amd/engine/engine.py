@@ -211,7 +211,11 @@ class _DecodeGraph:
 class Engine:
     def __init__(self, model: DecoderModel, *, num_pages: Optional[int] = None, max_tokens: Optional[int] = None,
                  page_tokens: int = 64, max_requests: int = 64, max_context: Optional[int] = None,
-                 poison_freed: bool = False, graphs: bool = True, streamed_weights: Optional[bool] = None):
+                 poison_freed: bool = False, graphs: bool = True, streamed_weights: Optional[bool] = None,
+                 cache_bits: Optional[int] = None):
+        """``cache_bits`` 4: keys and values are kept in 4 bits an element and a power of two for every 32 (``ops.FourBitPools``): 3.76
+        times the tokens in the memory of a bfloat16 cache, and as much less to read a step, for coarser keys and values (None: the
+        model's type).  Models of plain attention take it (``DecoderModel.cache_needs``)."""
         if model.embedding is None:
             raise ValueError("the model has no weights bound")
         if not torch.cuda.is_available() or model.device.type != "cuda":
@@ -228,7 +232,9 @@ class Engine:
             if max_tokens is None:
                 raise ValueError("give num_pages or max_tokens")
             num_pages = (max_tokens + page_tokens - 1) // page_tokens
-        self.pools = DevicePools(model.cache_needs(), self.dtype, self.device, num_pages, page_tokens, max_requests)
+        self.cache_bits = cache_bits
+        self.pools = DevicePools(model.cache_needs() if cache_bits is None else model.cache_needs(cache_bits), self.dtype, self.device,
+                                 num_pages, page_tokens, max_requests)
         model.keep_expert_copies()
         self.cache = CacheManager(self.pools.group_specs, max_requests, self.max_context)
         # With poison_freed every page is filled with NaN when its last holder lets go of it, whoever frees it

@@ -82,12 +82,13 @@ def _one_device(what: str, *tensors) -> None:
 def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_heads: int, kv_heads: int, head_dim: int, q_gain: Optional[torch.Tensor],
                             k_gain: Optional[torch.Tensor], eps: float, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
                             positions: torch.Tensor, row_entry: torch.Tensor, block_table: torch.Tensor, pools,
-                            out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                            write_cache: bool = True, out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
                             pairing: str = "half_split") -> torch.Tensor:
     """``qk_norm_rope_write`` for a cache of 4 bits an element: splits the fused projection, normalises and rotates q and k heads, writes
     k and v into the cache and returns q.  ``qkv`` is ``[rows, width]`` of q's type, or float32 (also as planes ``[p, rows, width]``
     whose sum is meant) with ``out_dtype`` naming the type of q.  Queries are rounded once, to that type; keys are computed in 64
-    bits up to their codes.  Rows at a position below 0, and rows whose place has no page, write nothing."""
+    bits up to their codes.  Rows at a position below 0, and rows whose place has no page, write nothing; without ``write_cache`` (a run
+    that reads what another one of the layer's wrote) none does."""
     what = "qk_norm_rope_write_4bit"
     planes = qkv.shape[0] if qkv.dim() == 3 else 1
     if qkv.dim() not in (2, 3) or qkv.shape[-1] != (q_heads + 2 * kv_heads) * head_dim or planes < 1:
@@ -108,7 +109,8 @@ def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_heads: int, kv_heads: int, head
             _CODES[kind], *_pool_args(what, pools), _dev(q_gain, f"{what}: q gain", None, (head_dim,)),
             _dev(k_gain, f"{what}: k gain", None, (head_dim,)), _code(q_gain, f"{what}: gain") if q_gain is not None else F32, float(eps),
             _dev(cos, f"{what}: cos", torch.float32), _dev(sin, f"{what}: sin", torch.float32), table_positions, rotary_dim, pairing_code,
-            *_row_args(what, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, head_dim, page_tokens)
+            *_row_args(what, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, head_dim, page_tokens,
+            1 if write_cache else 0)
     _one_device(what, qkv, out, *pools, q_gain, k_gain, cos, sin, positions, row_entry, block_table)
     if rows:
         call("leone_four_bit_fill", *args, _stream())

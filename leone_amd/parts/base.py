@@ -81,6 +81,8 @@ class KvNeed:
     value_dim: Optional[int] = None     # size of a value vector; None: the keys' size
     keep_first: int = 0                 # with a window: the first positions stay readable too (their pages are kept)
     chunk: int = 0                      # without one: keys are read within chunks of so many positions, counted from 0 (0: no chunks)
+    # Whether the mixer also takes its cache in 4 bits an element (``FourBitKvNeed``); says nothing about what is stored.
+    four_bits: bool = field(default=False, compare=False)
 
     paged = True
 
@@ -106,6 +108,42 @@ class KvNeed:
 
     def bytes_per_token(self, element_size: int) -> int:
         return self.kv_heads * (self.head_dim + (self.value_dim or self.head_dim)) * element_size
+
+    def in_four_bits(self) -> "FourBitKvNeed":
+        return FourBitKvNeed(self.kv_heads, self.head_dim, self.window, self.page_tokens)
+
+
+@dataclass(frozen=True)
+class FourBitKvNeed:
+    """The same vectors kept in blocks of 32 elements, 4 bits an element and a power of two a block (``ops.FourBitPools``): what a
+    ``KvNeed`` whose mixer says ``four_bits`` becomes in an engine that was asked for such a cache."""
+    kv_heads: int
+    head_dim: int
+    window: Optional[int] = None
+    page_tokens: Optional[int] = None
+
+    paged = True
+
+    def group_key(self):
+        return self
+
+    def allocate(self, pages: int, page_tokens: int, dtype: torch.dtype, device):
+        from .. import ops
+        if not ops.four_bit_supported(self.head_dim, page_tokens):
+            raise ValueError(f"a cache of 4 bits an element takes heads of a multiple of 32 elements up to 256 in pages of a multiple of 8 tokens, "
+                             f"not heads of {self.head_dim} in pages of {page_tokens}")
+        return ops.four_bit_pools(pages, self.kv_heads, self.head_dim, page_tokens, device)
+
+    def view(self, storage, block_table, page_tokens: int):
+        from .context import FourBitCacheView
+        return FourBitCacheView(writes=True, pools=storage, block_table=block_table, page_tokens=page_tokens)
+
+    def poison(self, storage, index: torch.Tensor) -> None:
+        for powers in (storage.k_powers, storage.v_powers):       # the power that stands for NaN
+            powers.index_fill_(0, index, 255)
+
+    def bytes_per_token(self, element_size: int) -> int:
+        return self.kv_heads * (self.head_dim + self.head_dim // 16)
 
 
 @dataclass(frozen=True)

@@ -71,5 +71,12 @@ class KvCacheView(CacheView):
 
 
 @dataclass
+class FourBitCacheView(CacheView):
+    pools: tuple = None                # ops.FourBitPools
+    block_table: torch.Tensor = None   # int32 [entries, max_blocks] of the layer's group
+    page_tokens: int = 0
+
+
+@dataclass
 class StateCacheView(CacheView):
     state: torch.Tensor = None         # [slots, *shape]: row entry_slots[e] belongs to entry e

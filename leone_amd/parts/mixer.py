@@ -9,7 +9,7 @@ import torch
 from .. import ops
 from ..weights.loader import MATRIX, VECTOR, TensorSpec
 from .base import CONVS, MIXERS, KvNeed, Part, PartSpec, RowTiling
-from .context import KvCacheView, StepContext
+from .context import FourBitCacheView, KvCacheView, StepContext
 from .position import rotation_of
 
 
@@ -146,7 +146,8 @@ class GqaAttention(Part):
     def cache_need(self):
         keys = KvNeed(self.kv_heads, self.head_dim, self.retain_window,
                       value_dim=self.value_dim if self.value_dim != self.head_dim else None,
-                      keep_first=self.retain_first if self.retain_window else 0, chunk=self.chunk)
+                      keep_first=self.retain_first if self.retain_window else 0, chunk=self.chunk,
+                      four_bits=not self.general and not self.keep_first and not self.retain_first and self.head_dim % 32 == 0)
         if self.conv is None:
             return keys
         return {"kv": keys, "conv": self.conv.cache_need()}
@@ -290,6 +291,13 @@ class GqaAttention(Part):
         cos, sin = rotation.cos, rotation.sin
         if cos is not None and step.max_position >= cos.shape[0]:
             raise ValueError(f"position {step.max_position} is beyond the rotary table of {cos.shape[0]} positions")
+        if isinstance(cache, FourBitCacheView):
+            q = ops.qk_norm_rope_write_4bit(qkv, self.q_heads, self.kv_heads, self.head_dim, self.q_gain, self.k_gain,
+                                            self.qk_norm_eps if self.qk_norm_eps is not None else 1.0, cos, sin, step.positions,
+                                            step.row_entry, cache.block_table, cache.pools, write_cache=cache.writes,
+                                            out_dtype=step.dtype, pairing=rotation.pairing)
+            attended = self._attend_four_bits(q, step, cache)
+            return ops.linear(attended, self.w_o, out_dtype=out_dtype, residual=residual, next_norm=next_norm)
         kernels = self.attention_kernels(step.dtype, cache.page_tokens, cache.block_table.shape[1])
         if step.decode_only and kernels["decode"] == "projected":
             # Single decoded tokens, every row another request: the attention kernel makes the heads itself.
@@ -366,6 +374,24 @@ class GqaAttention(Part):
             # the prompt kernel's rows; a gate for every element is a gate a head of one element
             heads, each = (self.q_heads * self.value_dim, 1) if self.gate_each else (self.q_heads, self.value_dim)
             ops.head_gate(out[:first], gate[:first], heads, each)
+        return out
+
+    def _attend_four_bits(self, q: torch.Tensor, step: StepContext, cache: FourBitCacheView) -> torch.Tensor:
+        """The same over a cache of 4 bits an element."""
+        window = int(self.window or 0)
+        where = (cache.block_table, self.q_heads, self.scale, window)
+        if not ops.four_bit_decode_supported(q.dtype, self.head_dim, cache.page_tokens):
+            return ops.attention_rows_4bit(q, cache.pools, step.positions, step.row_entry, *where, max_context=step.max_position + 1)
+        first = 0
+        out = torch.empty_like(q)
+        tiled = step.tiled.get(self.row_tiling())
+        if tiled is not None and tiled.rows and ops.four_bit_prefill_supported(q.dtype, self.head_dim, cache.page_tokens):
+            ops.attention_prefill_4bit(q, out, cache.pools, step.positions, tiled.tiles, *where,
+                                       mean_keys=tiled.mean_keys or step.max_position + 1, covered_rows=tiled.rows)
+            first = tiled.rows
+        if first < step.rows:
+            ops.attention_decode_4bit(q[first:], cache.pools, step.positions[first:], step.row_entry[first:], *where,
+                                      max_context=step.max_position + 1, out=out[first:])
         return out
 
     def _attend_talking(self, q: torch.Tensor, step: StepContext, cache: KvCacheView, window: int) -> torch.Tensor:

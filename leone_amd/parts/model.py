@@ -273,10 +273,13 @@ class DecoderModel:
         return sum(self.weight_accounting(rows=rows)["decode"].values())
 
     # ---- cache ---------------------------------------------------------------
-    def cache_needs(self) -> Dict[int, object]:
+    def cache_needs(self, bits: Optional[int] = None) -> Dict[int, object]:
         """Cache slot -> what the layer runs on it need (one need per slot).  A layer that needs several kinds
         of storage (``cache_need()`` answers with a dict, see ``parts.base.flatten_needs``) gets one slot for
-        each, keyed (the run's slot, *names)."""
+        each, keyed (the run's slot, *names).  ``bits`` 4: keys and values in 4 bits an element (``FourBitKvNeed``), which
+        every layer that caches a token's vectors has to take; state a request keeps stays what it is."""
+        if bits not in (None, 4):
+            raise ValueError(f"a cache of {bits} bits an element is not known; 4, or the model's own type (None)")
         needs: Dict[object, object] = {}
         writers: Dict[object, int] = {}
         for run in self.schedule:
@@ -295,11 +298,16 @@ class DecoderModel:
                     raise ValueError(f"cache slot {key} is shared by layers with different needs")
                 if lent is not None and key not in needs:
                     raise ValueError(f"layer {run.layer} borrows cache slot {key}, which no earlier run keeps")
+                if bits is not None and getattr(leaf, "paged", False) and not getattr(leaf, "four_bits", False):
+                    raise ValueError(f"layer {run.layer} does not take its cache in 4 bits an element: attention with norms of single heads, a "
+                                     f"rotation and a window does, on keys and values of its own and of one size")
                 needs[key] = leaf
             writers[run.cache] = writers.get(run.cache, 0) + (1 if run.writes else 0)
         for slot, count in writers.items():
             if count != 1:
                 raise ValueError(f"cache slot {slot} must have exactly one writing run, found {count}")
+        if bits is not None:
+            needs = {key: leaf.in_four_bits() if getattr(leaf, "four_bits", False) else leaf for key, leaf in needs.items()}
         return needs
 
     @staticmethod
