@@ -519,59 +519,84 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
 
 
 
-// The merge of shares: a wave a row and head; lane s has share s's maximum and sum.
+// The merge of shares.  kGroup neighbouring lanes have a row and head, four elements each; between them they hold the shares' maxima and
+// sums and hand the weights round, four shares' sums on their way at a time.
 constexpr int kMergeThreads = 256;
+constexpr int kMergeAhead = 4;
 
-template <typename T>
+template <int kGroup, typename T>
 __global__ void __launch_bounds__(kMergeThreads)
 four_bit_merge_kernel(const float* __restrict__ part_acc, const float* __restrict__ part_ml, T* __restrict__ out, long items, int q_heads, int dim,
                       int splits, const int* __restrict__ tiles) {
-    long row_head = static_cast<long>(blockIdx.x) * (kMergeThreads / kWave) + threadIdx.x / kWave;
-    if (row_head >= items) return;
+    constexpr int kEach = kShares / kGroup;                      // shares whose weights a lane holds
+    const int lane = threadIdx.x % kGroup;
+    long item = (static_cast<long>(blockIdx.x) * kMergeThreads + threadIdx.x) / kGroup;
+    bool exists = item < items;
+    if (!exists) item = 0;                                       // (every lane goes along: weights are handed round)
     if (tiles != nullptr) {
-        const long place = row_head / q_heads;
+        const long place = item / q_heads;
         const int* tile = tiles + 3 * (place / kTileRows);
         const int r = static_cast<int>(place % kTileRows);
-        if (r >= tile[2]) return;
-        row_head = (static_cast<long>(tile[1]) + r) * q_heads + row_head % q_heads;
+        exists &= r < tile[2];
+        item = exists ? (static_cast<long>(tile[1]) + r) * q_heads + item % q_heads : 0;
     }
-    const int lane = threadIdx.x % kWave;
-    const float m = lane < splits ? part_ml[2 * (row_head * splits + lane)] : -INFINITY;
-    const float l = lane < splits ? part_ml[2 * (row_head * splits + lane) + 1] : 0.f;
-    const float top = wave_max(m);
-    const float by = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
-    const float den = wave_sum(m == -INFINITY ? 0.f : l * by);
-    const bool mine = 4 * lane < dim;                            // (the other lanes go along: every lane's weight is asked for below)
-    const int d = mine ? 4 * lane : 0;
+    const float* ml = part_ml + 2 * item * splits;
+    float m[kEach], by[kEach], top = -INFINITY, den = 0.f;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        m[k] = k * kGroup + lane < splits ? ml[2 * (k * kGroup + lane)] : -INFINITY;
+        by[k] = k * kGroup + lane < splits ? ml[2 * (k * kGroup + lane) + 1] : 0.f;
+        top = fmaxf(top, m[k]);
+    }
+    top = join_span<kGroup>(top, [](float a, float b) { return fmaxf(a, b); });
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        const float w = m[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[k] - top);
+        den += m[k] == -INFINITY ? 0.f : by[k] * w;
+        by[k] = w;
+    }
+    den = join_span<kGroup>(den, [](float a, float b) { return a + b; });
+    const bool mine = 4 * lane < dim;
+    const float* from = part_acc + item * splits * dim + (mine ? 4 * lane : 0);
     floatx4 num = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < splits; s0 += 8) {
-        floatx4 x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)                          // (a share behind the last is the last again and weighs nothing)
-            x[i] = *reinterpret_cast<const floatx4*>(part_acc + (row_head * splits + min(s0 + i, splits - 1)) * dim + d);
+    for (int k = 0; k < kEach; ++k) {
+        for (int s0 = k * kGroup; s0 < min(splits, (k + 1) * kGroup); s0 += kMergeAhead) {
+            floatx4 x[kMergeAhead];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float w = s0 + i < splits ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, by), s0 + i)) : 0.f;
-            if (w > 0.f) {                                   // an empty share's sums were never written
+            for (int i = 0; i < kMergeAhead; ++i)                // (a share behind the last is the last again and weighs nothing)
+                x[i] = *reinterpret_cast<const floatx4*>(from + static_cast<long>(min(s0 + i, splits - 1)) * dim);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) num[e] += x[i][e] * w;
+            for (int i = 0; i < kMergeAhead; ++i) {
+                const float w = s0 + i < splits ? __shfl(by[k], (s0 + i) % kGroup, kGroup) : 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) num[e] = w > 0.f ? fmaf(x[i][e], w, num[e]) : num[e];   // (an empty share's sums were never written)
             }
         }
     }
-    if (!mine) return;
-    T* to = out + row_head * dim + d;
+    if (!exists || !mine) return;
+    T* to = out + item * dim + 4 * lane;
 #pragma unroll
     for (int e = 0; e < 4; ++e) to[e] = from_float<T>(top == -INFINITY ? 0.f : num[e] / den);
+}
+
+template <typename T>
+static void launch_merge(const float* part_acc, const float* part_ml, T* out, long items, int q_heads, int dim, int splits, const int* tiles,
+                         hipStream_t stream) {
+#define LEONE_MERGE(GROUP)                                                                                                                    \
+    four_bit_merge_kernel<GROUP, T><<<ceil_div(items * GROUP, kMergeThreads), kMergeThreads, 0, stream>>>(part_acc, part_ml, out, items, q_heads, \
+                                                                                                         dim, splits, tiles)
+    if (dim <= 64) LEONE_MERGE(16);
+    else if (dim <= 128) LEONE_MERGE(32);
+    else LEONE_MERGE(64);
+#undef LEONE_MERGE
 }
 
 void merge_four_bit_shares(const float* part_acc, const float* part_ml, void* out, int dtype, long rows, int q_heads, int dim, int splits,
                            const int* tiles, hipStream_t stream) {
     const long items = rows * q_heads;
-    const int blocks = ceil_div(items, kMergeThreads / kWave);
-    if (dtype == kF32)
-        four_bit_merge_kernel<float><<<blocks, kMergeThreads, 0, stream>>>(part_acc, part_ml, static_cast<float*>(out), items, q_heads, dim, splits, tiles);
-    else
-        four_bit_merge_kernel<bf16_t><<<blocks, kMergeThreads, 0, stream>>>(part_acc, part_ml, static_cast<bf16_t*>(out), items, q_heads, dim, splits, tiles);
+    if (dtype == kF32) launch_merge(part_acc, part_ml, static_cast<float*>(out), items, q_heads, dim, splits, tiles, stream);
+    else launch_merge(part_acc, part_ml, static_cast<bf16_t*>(out), items, q_heads, dim, splits, tiles, stream);
 }
 
 }  // namespace leone

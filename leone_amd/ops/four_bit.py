@@ -46,37 +46,60 @@ def four_bit_pools(pages: int, kv_heads: int, head_dim: int, page_tokens: int, d
 
 def four_bit_dims(pools) -> tuple:
     """(pages, kv_heads, page_tokens, head_dim) of a cache of 4 bits an element."""
-    if len(pools) != 4 or any(p.dim() != d for p, d in zip(pools, (5, 4, 6, 5))):
-        raise KernelError("a cache of 4 bits an element is four tensors: key codes, key powers, value codes, value powers")
-    pages, kv_heads, blocks, page_tokens, _ = pools[0].shape
+    try:
+        k_codes, k_powers, v_codes, v_powers = pools
+        pages, kv_heads, blocks, page_tokens, block_bytes = k_codes.shape
+    except (ValueError, AttributeError, TypeError):
+        raise KernelError("a cache of 4 bits an element is four tensors: key codes, key powers, value codes, value powers") from None
     dim = blocks * BLOCK
-    want = ((pages, kv_heads, blocks, page_tokens, 16), (pages, kv_heads, page_tokens, blocks),
-            (pages, kv_heads, page_tokens // 4, dim // 8, 4, 4), (pages, kv_heads, page_tokens // 4, blocks, 4))
-    found = tuple(tuple(p.shape) for p in pools)
-    if found != want or not four_bit_supported(dim, page_tokens):
-        raise KernelError(f"pools of shapes {found} are no cache of 4 bits an element")
+    if (block_bytes != 16 or k_powers.shape != (pages, kv_heads, page_tokens, blocks)
+            or v_codes.shape != (pages, kv_heads, page_tokens // 4, dim // 8, 4, 4)
+            or v_powers.shape != (pages, kv_heads, page_tokens // 4, blocks, 4) or not four_bit_supported(dim, page_tokens)):
+        raise KernelError(f"pools of shapes {tuple(tuple(p.shape) for p in pools)} are no cache of 4 bits an element")
     return pages, kv_heads, page_tokens, dim
 
 
-def _pool_args(what: str, pools) -> tuple:
-    return tuple(_dev(p, f"{what}: {name}", torch.uint8) for p, name in zip(pools, FourBitPools._fields)) + (pools[0].shape[0],)
+# A call's time on the host counts where a step is issued kernel by kernel (and is what a short one waits for), so the checks below
+# ask each tensor once and put their messages together only when something is refused.
+def _current(what: str, t: torch.Tensor) -> int:
+    """The current device, which the tensors have to be on: a launch goes to its stream."""
+    device = t.get_device()
+    if device < 0:
+        raise KernelError(f"{what}: tensor is on {t.device}; the kernels run on the GPU only")
+    if device != torch.cuda.current_device():
+        raise KernelError(f"{what}: tensors on {t.device}, which is not the current device")
+    return device
 
 
-def _row_args(what: str, rows: int, positions: torch.Tensor, row_entry: torch.Tensor, block_table: torch.Tensor) -> tuple:
+def _at(what: str, name: str, t: torch.Tensor, device: int, dtype: torch.dtype, shape: tuple) -> int:
+    """The address of an operand that is as it has to be."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr()
+    _dev(t, f"{what}: {name}", dtype, shape)
+    raise KernelError(f"{what}: {name} is on {t.device}, the others on cuda:{device}; one device is needed")
+
+
+def _pools_at(what: str, pools, device: int) -> tuple:
+    """Addresses and pages of pools whose shapes ``four_bit_dims`` has seen."""
+    kc, kp, vc, vp = pools
+    if (kc.dtype is kp.dtype is vc.dtype is vp.dtype is torch.uint8 and kc.get_device() == kp.get_device() == vc.get_device() == vp.get_device() == device
+            and kc.is_contiguous() and kp.is_contiguous() and vc.is_contiguous() and vp.is_contiguous()):
+        return kc.data_ptr(), kp.data_ptr(), vc.data_ptr(), vp.data_ptr(), len(kc)
+    return tuple(_at(what, name, p, device, torch.uint8, p.shape) for p, name in zip(pools, FourBitPools._fields)) + (len(kc),)
+
+
+def _rows_at(what: str, device: int, rows: int, positions: torch.Tensor, row_entry: torch.Tensor, block_table: torch.Tensor) -> tuple:
+    if positions is None or row_entry is None or block_table is None:
+        raise KernelError(f"{what}: positions, a row map and a block table are needed")
+    int32, wanted = torch.int32, (rows,)
+    if (positions.dtype is row_entry.dtype is block_table.dtype is int32 and positions.shape == wanted and row_entry.shape == wanted
+            and positions.get_device() == row_entry.get_device() == block_table.get_device() == device and block_table.dim() == 2
+            and positions.is_contiguous() and row_entry.is_contiguous() and block_table.is_contiguous()):
+        return positions.data_ptr(), row_entry.data_ptr(), block_table.data_ptr(), block_table.shape[1], block_table.shape[0]
     if block_table.dim() != 2:
         raise KernelError(f"{what}: a block table is int32 [entries, blocks]")
-    return (_dev(positions, f"{what}: positions", torch.int32, (rows,)), _dev(row_entry, f"{what}: row map", torch.int32, (rows,)),
-            _dev(block_table, f"{what}: block table", torch.int32), block_table.shape[1], block_table.shape[0])
-
-
-def _one_device(what: str, *tensors) -> None:
-    """A launch goes to the current device's stream: tensors of another device, or of several, are refused."""
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise KernelError(f"{what}: tensors on {', '.join(sorted(str(d) for d in devices))}; one device is needed")
-    device = next(iter(devices))
-    if device.type == "cuda" and device.index is not None and device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: tensors on {device}, which is not the current device")
+    return (_at(what, "positions", positions, device, int32, wanted), _at(what, "row map", row_entry, device, int32, wanted),
+            _at(what, "block table", block_table, device, int32, block_table.shape), block_table.shape[1], block_table.shape[0])
 
 
 def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_heads: int, kv_heads: int, head_dim: int, q_gain: Optional[torch.Tensor],
@@ -105,13 +128,16 @@ def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_heads: int, kv_heads: int, head
         raise KernelError(f"{what}: q and k gains must come together in one type")
     if out is None:
         out = torch.empty((rows, q_heads * head_dim), dtype=kind, device=qkv.device)
-    args = (_dev(qkv, f"{what}: qkv"), _code(qkv, what), planes, rows * width, width, _dev(out, f"{what}: q out", kind, (rows, q_heads * head_dim)),
-            _CODES[kind], *_pool_args(what, pools), _dev(q_gain, f"{what}: q gain", None, (head_dim,)),
-            _dev(k_gain, f"{what}: k gain", None, (head_dim,)), _code(q_gain, f"{what}: gain") if q_gain is not None else F32, float(eps),
-            _dev(cos, f"{what}: cos", torch.float32), _dev(sin, f"{what}: sin", torch.float32), table_positions, rotary_dim, pairing_code,
-            *_row_args(what, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, head_dim, page_tokens,
-            1 if write_cache else 0)
-    _one_device(what, qkv, out, *pools, q_gain, k_gain, cos, sin, positions, row_entry, block_table)
+    device = _current(what, qkv)
+    float32 = torch.float32
+    args = (_at(what, "qkv", qkv, device, qkv.dtype, qkv.shape), _CODES[qkv.dtype], planes, rows * width, width,
+            _at(what, "q out", out, device, kind, (rows, q_heads * head_dim)), _CODES[kind], *_pools_at(what, pools, device),
+            0 if q_gain is None else _at(what, "q gain", q_gain, device, q_gain.dtype, (head_dim,)),
+            0 if k_gain is None else _at(what, "k gain", k_gain, device, k_gain.dtype, (head_dim,)),
+            F32 if q_gain is None else _code(q_gain, "qk_norm_rope_write_4bit: gain"), eps,
+            0 if cos is None else _at(what, "cos", cos, device, float32, cos.shape), 0 if sin is None else _at(what, "sin", sin, device, float32, sin.shape),
+            table_positions, rotary_dim, pairing_code, *_rows_at(what, device, rows, positions, row_entry, block_table), rows, q_heads, kv_heads,
+            head_dim, page_tokens, 1 if write_cache else 0)
     if rows:
         call("leone_four_bit_fill", *args, _stream())
     return out
@@ -122,12 +148,12 @@ def cache_rows_4bit(pools, positions: torch.Tensor, row_entry: torch.Tensor, blo
     times its power is a bfloat16 as it is).  Rows without a page give NaN."""
     what = "cache_rows_4bit"
     pages, kv_heads, page_tokens, dim = four_bit_dims(pools)
+    device = _current(what, positions)
     rows = positions.shape[0]
     k = torch.empty((rows, kv_heads * dim), dtype=torch.bfloat16, device=positions.device)
     v = torch.empty_like(k)
-    args = (*_pool_args(what, pools), *_row_args(what, rows, positions, row_entry, block_table), _dev(k, what), _dev(v, what), rows, kv_heads, dim,
-            page_tokens)
-    _one_device(what, *pools, positions, row_entry, block_table)
+    args = (*_pools_at(what, pools, device), *_rows_at(what, device, rows, positions, row_entry, block_table), k.data_ptr(), v.data_ptr(), rows,
+            kv_heads, dim, page_tokens)
     if rows:
         call("leone_four_bit_rows", *args, _stream())
     return k, v
@@ -142,18 +168,21 @@ def _attention_shape(what: str, q: torch.Tensor, pools, q_heads: int, window: in
     return kv_heads, page_tokens, dim
 
 
-def _workspace(rows: int, q_heads: int, dim: int, splits: int, device) -> tuple:
-    """Partial results of rows whose keys are shared out, and their maxima and sums."""
+def _shares_at(rows: int, q_heads: int, dim: int, splits: int, device) -> tuple:
+    """(a tensor to hold on to, partial results of rows whose keys are shared out, their maxima and sums)."""
     if splits == 1:
-        return None, None
-    return (torch.empty((rows * q_heads * splits * dim,), dtype=torch.float32, device=device),
-            torch.empty((rows * q_heads * splits * 2,), dtype=torch.float32, device=device))
+        return None, 0, 0
+    shares = rows * q_heads * splits
+    held = torch.empty((shares * (dim + 2),), dtype=torch.float32, device=device)
+    at = held.data_ptr()
+    return held, at, at + 4 * shares * dim
 
 
 def four_bit_row_splits(blocks: int, keys: int, units: int = 256) -> int:
     """How many workgroups share a row's keys in ``attention_rows_4bit``, where ``blocks`` workgroups would have them all: as many as
-    leave none of the chip's units idle, but no fewer than 64 keys for each of a workgroup's four waves."""
-    return max(1, min(units // max(1, blocks), keys // 256, 64))
+    leave none of the chip's units idle, but no more than give each of their four waves 64 keys (4 rows of 501 to 777 keys, 16 blocks:
+    21 us with 3, where some waves have two tiles, 14.1 with 4, 14.4 with 16)."""
+    return max(1, min(units // max(1, blocks), -(-keys // 256), 64))
 
 
 def attention_rows_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_entry: torch.Tensor, block_table: torch.Tensor, q_heads: int,
@@ -171,11 +200,11 @@ def attention_rows_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_ent
         splits = four_bit_row_splits(rows * kv_heads * (-(-(q_heads // kv_heads) // 4)), keys, compute_units(q.device))
     if out is None:
         out = torch.empty_like(q)
-    part_acc, part_ml = _workspace(rows, q_heads, dim, splits, q.device)
-    args = (_dev(q, f"{what}: q"), _dev(out, f"{what}: out", q.dtype, q.shape), _code(q, what), *_pool_args(what, pools),
-            *_row_args(what, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, dim, page_tokens, float(scale), int(window),
-            int(splits), _dev(part_acc, what), _dev(part_ml, what))
-    _one_device(what, q, out, *pools, positions, row_entry, block_table)
+    device = _current(what, q)
+    held, part_acc, part_ml = _shares_at(rows, q_heads, dim, splits, q.device)
+    args = (_at(what, "q", q, device, q.dtype, q.shape), _at(what, "out", out, device, q.dtype, q.shape), _code(q, what),
+            *_pools_at(what, pools, device), *_rows_at(what, device, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, dim, page_tokens,
+            scale, window, splits, part_acc, part_ml)
     if rows:
         call("leone_four_bit_attend_rows", *args, _stream())
     return out
@@ -211,11 +240,11 @@ def attention_decode_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_e
                                         compute_units(q.device))
     if out is None:
         out = torch.empty_like(q)
-    part_acc, part_ml = _workspace(rows, q_heads, dim, splits, q.device)
-    args = (_dev(q, f"{what}: q"), _dev(out, f"{what}: out", q.dtype, q.shape), *_pool_args(what, pools),
-            *_row_args(what, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, dim, page_tokens, float(scale), int(window),
-            int(splits), _dev(part_acc, what), _dev(part_ml, what))
-    _one_device(what, q, out, *pools, positions, row_entry, block_table)
+    device = _current(what, q)
+    held, part_acc, part_ml = _shares_at(rows, q_heads, dim, splits, q.device)
+    args = (_at(what, "q", q, device, q.dtype, q.shape), _at(what, "out", out, device, q.dtype, q.shape), *_pools_at(what, pools, device),
+            *_rows_at(what, device, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, dim, page_tokens, scale, window, splits,
+            part_acc, part_ml)
     if rows:
         call("leone_four_bit_decode", *args, _stream())
     return out
@@ -246,12 +275,12 @@ def attention_prefill_4bit(q: torch.Tensor, out: torch.Tensor, pools, positions:
     covered = rows if covered_rows is None else covered_rows
     if not 0 <= covered <= rows:
         raise KernelError(f"{what}: {covered} covered rows of {rows}")
-    part_acc, part_ml = _workspace(covered, q_heads, dim, splits, q.device)
-    args = (_dev(q, f"{what}: q"), _dev(out, f"{what}: out", q.dtype, q.shape), *_pool_args(what, pools),
-            _dev(positions, f"{what}: positions", torch.int32, (rows,)), _dev(tiles, f"{what}: tiles", torch.int32), groups,
-            _dev(block_table, f"{what}: block table", torch.int32), block_table.shape[1], block_table.shape[0], q_heads, kv_heads, dim, page_tokens,
-            float(scale), int(window), int(splits), _dev(part_acc, what), _dev(part_ml, what))
-    _one_device(what, q, out, *pools, positions, tiles, block_table)
+    device = _current(what, q)
+    held, part_acc, part_ml = _shares_at(covered, q_heads, dim, splits, q.device)
+    args = (_at(what, "q", q, device, q.dtype, q.shape), _at(what, "out", out, device, q.dtype, q.shape), *_pools_at(what, pools, device),
+            _at(what, "positions", positions, device, torch.int32, (rows,)), _at(what, "tiles", tiles, device, torch.int32, tiles.shape), groups,
+            _at(what, "block table", block_table, device, torch.int32, block_table.shape), block_table.shape[1], block_table.shape[0], q_heads,
+            kv_heads, dim, page_tokens, scale, window, splits, part_acc, part_ml)
     if groups and covered:
         call("leone_four_bit_prefill", *args, _stream())
     return out
