@@ -46,6 +46,13 @@ constexpr int kPromptUnits = 256;                     // compute units: workgrou
 // Row of a pass's first product <-> key of the pass.
 __device__ inline int pass_key(int x) { return (x & 0x13) | ((x & 4) << 1) | ((x & 8) >> 1); }
 
+// A barrier that orders shared memory alone: __syncthreads waits for every load in flight, the stages that are on their way among them.
+__device__ inline void shared_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 template <int kD>
 struct PromptStage {
     uint4 keys[kD / kBlock * kStageKeys];             // [half][block][row of the first product]
@@ -220,7 +227,7 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
             }
         };
         // The values on their way into shared memory: by token, two elements at a time, then by element.
-        auto deposit = [&](int t, PromptStage<kD>* to) {
+        auto deposit = [&](int note, PromptStage<kD>* to) {
             if (brings) {
                 to->keys[tid] = k_codes;
                 unsigned nan_tokens = 0;
@@ -232,8 +239,8 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (nan_tokens >> i & 1u) words[i] = 0, powers = (powers & ~(0xffu << (8 * i))) | (0x7fu << (8 * i));
-                    nan_seen[t % 3] = 1;
-                    atomicOr(&nan_keys[t % 3][v_eight / 4], static_cast<unsigned long long>(nan_tokens) << v_key);
+                    nan_seen[note] = 1;
+                    atomicOr(&nan_keys[note][v_eight / 4], static_cast<unsigned long long>(nan_tokens) << v_key);
                 }
                 float power[4];
 #pragma unroll
@@ -318,11 +325,10 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
             const int at = 32 * dt + 8 * (v / 4) + 4 * h + v % 4;
             return (at % kEights) / 4;
         };
-        auto spoil = [&](int t) {
-            if (nan_seen[t % 3] == 0) return;
+        auto spoil = [&](int t, int note) {
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
-                const unsigned long long keys = nan_keys[t % 3][b];
+                const unsigned long long keys = nan_keys[note][b];
                 if (keys == 0) continue;                         // (the same for the workgroup)
                 const int first = max(row_lo - t * kStageKeys, 0), last = min(row_pos - t * kStageKeys, kStageKeys - 1);
                 unsigned long long seen = last >= first ? (~0ull >> (63 - last + first)) << first : 0ull;
@@ -344,34 +350,38 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
         // where there is no further: see `find`.)
         fetch(t_begin, find(t_begin));
         Pages ahead = find(min(t_begin + 1, t_end - 1));
-        deposit(t_begin, &stages[0]);
+        deposit(0, &stages[0]);
         unsigned k_powers_ready[2] = {k_powers_next[0], k_powers_next[1]};
         k_powers[0] = k_powers_next[0], k_powers[1] = k_powers_next[1];
         fetch(min(t_begin + 1, t_end - 1), ahead);
         ahead = find(min(t_begin + 2, t_end - 1));
-        __syncthreads();
-        auto round = [&](const PromptStage<kD>* __restrict__ reading, PromptStage<kD>* __restrict__ writing, int t) {
+        shared_barrier();
+        // `note`, `next_note`, `old_note`: whose NaN keys are read, written and cleared in this round
+        auto round = [&](const PromptStage<kD>* __restrict__ reading, PromptStage<kD>* __restrict__ writing, int t, int note, int next_note, int old_note) {
+            const int any_nan = nan_seen[note];                   // (asked for with the keys, used behind them)
             const bool plain = t >= plain_begin && t < plain_end;    // nothing to mask: most stages of a long context
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int key0 = t * kStageKeys + half * kPassKeys;
                 if (plain || (key0 < key_hi && key0 + kPassKeys > key_lo)) pass(reading, key0, half, plain);
                 if (half == 0) {
-                    if (t + 1 < t_end) deposit(t + 1, writing);
+                    if (t + 1 < t_end) deposit(next_note, writing);
                     k_powers_ready[0] = k_powers_next[0], k_powers_ready[1] = k_powers_next[1];
                     fetch(min(t + 2, t_end - 1), ahead);
                     ahead = find(min(t + 3, t_end - 1));
                 }
             }
-            spoil(t);
-            if (tid < kBlocks) nan_keys[(t + 2) % 3][tid] = 0;
-            if (tid == 0) nan_seen[(t + 2) % 3] = 0;
+            if (any_nan != 0) spoil(t, note);
+            if (tid < kBlocks) nan_keys[old_note][tid] = 0;
+            if (tid == 0) nan_seen[old_note] = 0;
         };
+        int note = 0;
         for (int t = t_begin; t < t_end; ++t) {
-            const int cur = (t - t_begin) & 1;
-            round(&stages[cur], &stages[cur ^ 1], t);
+            const int cur = (t - t_begin) & 1, next_note = note == 2 ? 0 : note + 1, old_note = note == 0 ? 2 : note - 1;
+            round(&stages[cur], &stages[cur ^ 1], t, note, next_note, old_note);
+            note = next_note;
             k_powers[0] = k_powers_ready[0], k_powers[1] = k_powers_ready[1];
-            __syncthreads();
+            shared_barrier();
         }
     }
     __syncthreads();
