@@ -203,7 +203,7 @@ four_bit_attend_rows_kernel(const T* __restrict__ q, T* __restrict__ out, FourBi
 // ---- single tokens on the matrix cores -----------------------------------------------------------------------------------
 constexpr int kDecodeWaves = 4;
 constexpr int kDecodeThreads = kDecodeWaves * kWave;
-constexpr int kTileKeys = 32;
+constexpr int kTileKeys = 32;     // (of 64 a lone wave is a fifth faster, but two a SIMD fit instead of three: 64 rows of 300 to 8,191 keys level, 2 of 100 10 % slower)
 
 template <int kD, bool kOnePage>
 __global__ void __launch_bounds__(kDecodeThreads, kD <= 128 ? 3 : 2)
@@ -212,6 +212,7 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
                        int kv_heads, int page_shift, float to_log2, int window, int splits, float* __restrict__ part_acc,
                        float* __restrict__ part_ml) {
     constexpr int kCols = decode_columns(kD);
+    constexpr int kSubs = kTileKeys / 16;                         // products of sixteen keys a tile
     constexpr int kSteps = kD <= 128 ? 1 : kD / 128;              // of 128 elements
     constexpr int kParts = kD <= 64 ? 1 : 2;                      // products a step: heads of 64 hold both parts of a query in one
     constexpr int kVLoads = kD <= 128 ? 1 : kD / 128;             // eights a lane has of each of its tokens
@@ -222,7 +223,11 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
     const int group = q_heads / kv_heads, col_tiles = (group + kCols - 1) / kCols;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
     const int c = lane & 15, g = lane >> 4;
-    const int row = blockIdx.x, kvh = blockIdx.y / col_tiles, col0 = (blockIdx.y - kvh * col_tiles) * kCols;
+    // Rows differ in length, and a unit whose two workgroups are long ones is what the launch waits for: workgroups 256 apart share a unit, and
+    // with the rows of every second half of the heads in falling order they are two rows', not two heads' of one (64 rows of 300
+    // to 8,191 keys in no order, 8 kv heads: 63.8 us, 70.7 in the grid's order).
+    const int row = blockIdx.y >= gridDim.y / 2 ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+    const int kvh = blockIdx.y / col_tiles, col0 = (blockIdx.y - kvh * col_tiles) * kCols;
     const int cols = min(kCols, group - col0), split = blockIdx.z;
     const int entry = row_entry[row], pos = positions[row];
     const int all = entry >= 0 && entry < entries ? pos + 1 : 0;
@@ -241,12 +246,12 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
     // (Every call of `issue` is the same loads whatever the tile, also behind the last: after a load that may or may not have been
     // issued the compiler waits for all.  Addresses are a base that is the same for the wave and a lane's 32-bit offset that does not
     // change: with 64-bit products for every load a tile cost 1,700 cycles of a wave, half of it scalar arithmetic.)
-    constexpr int kPages = kOnePage ? 1 : 2;
+    constexpr int kPages = kOnePage ? 1 : kSubs;
     struct Tile {
-        uint4 k[2][kSteps];                                       // key 16 half + c
-        unsigned k_power[2][kSteps];
-        uint4 v[2][kVLoads];                                      // keys 16 half + 4 g .. + 3
-        unsigned v_power[2][kVLoads];
+        uint4 k[kSubs][kSteps];                                   // key 16 sub + c
+        unsigned k_power[kSubs][kSteps];
+        uint4 v[kSubs][kVLoads];                                  // keys 16 sub + 4 g .. + 3
+        unsigned v_power[kSubs][kVLoads];
         int page[kPages];
     };
     struct Pages {
@@ -268,11 +273,11 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
     };
     auto issue = [&](int t, const Pages& found, Tile& r) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int i = kOnePage ? 0 : half;
+        for (int sub = 0; sub < kSubs; ++sub) {
+            const int i = kOnePage ? 0 : sub;
             r.page[i] = found.id[i];
             const unsigned page = static_cast<unsigned>(found.id[i]) < static_cast<unsigned>(pools.pages) ? found.id[i] : 0;
-            const unsigned token = (t * kTileKeys + 16 * half) & page_mask;
+            const unsigned token = (t * kTileKeys + 16 * sub) & page_mask;
             const unsigned long long codes = static_cast<unsigned long long>(page) * code_stride, powers = static_cast<unsigned long long>(page) * power_stride;
             const uint8_t* kc = k_codes + codes + 16 * token;                             // (a block of so many tokens' keys)
             const uint8_t* kp = k_powers + powers + kD / kBlock * token;
@@ -280,13 +285,13 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
             const uint8_t* vp = v_powers + powers + kD / kBlock * token;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                r.k[half][s] = load_streamed16(kc + (k_code_at + s * four_bit_key(0, 4, page_tokens)));
-                r.k_power[half][s] = kp[k_power_at + 4 * s];
+                r.k[sub][s] = load_streamed16(kc + (k_code_at + s * four_bit_key(0, 4, page_tokens)));
+                r.k_power[sub][s] = kp[k_power_at + 4 * s];
             }
 #pragma unroll
             for (int s = 0; s < kVLoads; ++s) {
-                r.v[half][s] = load_streamed16(vc + (v_code_at + s * four_bit_value(0, 16, kD)));
-                r.v_power[half][s] = *reinterpret_cast<const unsigned*>(vp + (v_power_at + s * four_bit_value_power(0, 4, kD)));
+                r.v[sub][s] = load_streamed16(vc + (v_code_at + s * four_bit_value(0, 16, kD)));
+                r.v_power[sub][s] = *reinterpret_cast<const unsigned*>(vp + (v_power_at + s * four_bit_value_power(0, 4, kD)));
             }
         }
     };
@@ -343,45 +348,46 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
 
     auto finish = [&](int tile, Tile& r) {
         const int key0 = tile * kTileKeys;
-        bool no_page[2];
+        bool no_page[kSubs], full = key0 >= lo && key0 + kTileKeys <= n;          // the same for the whole wave
 #pragma unroll
-        for (int half = 0; half < 2; ++half) no_page[half] = static_cast<unsigned>(r.page[kOnePage ? 0 : half]) >= static_cast<unsigned>(pools.pages);
-        const bool full = key0 >= lo && key0 + kTileKeys <= n && !no_page[0] && !no_page[1];      // the same for the whole wave
-        // ---- scores of keys 4 g .. + 3 of both halves for column c
-        floatx4 s4[2];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            s4[half] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                s4[half] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(low_half(r.k[half][s]), query[s][0], s4[half], 4, 0, 0,
-                                                                            static_cast<int>(r.k_power[half][s]), 0, power_high);
-                if constexpr (kParts == 2)
-                    s4[half] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(low_half(r.k[half][s]), query[s][kParts - 1], s4[half], 4, 0, 0,
-                                                                                static_cast<int>(r.k_power[half][s]), 0, power_low);
-            }
+        for (int sub = 0; sub < kSubs; ++sub) {
+            no_page[sub] = static_cast<unsigned>(r.page[kOnePage ? 0 : sub]) >= static_cast<unsigned>(pools.pages);
+            full &= !no_page[sub];
         }
-        float sc[8];
+        // ---- scores of keys 16 sub + 4 g .. + 3 for column c
+        floatx4 s4[kSubs];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sc[j] = s4[j / 4][j % 4] * to_log2;
+        for (int sub = 0; sub < kSubs; ++sub) s4[sub] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+            for (int part = 0; part < kParts; ++part)             // (the sixteens in turn: no product waits for the one before)
+#pragma unroll
+                for (int sub = 0; sub < kSubs; ++sub)
+                    s4[sub] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(low_half(r.k[sub][s]), query[s][part], s4[sub], 4, 0, 0,
+                                                                              static_cast<int>(r.k_power[sub][s]), 0, part == 0 ? power_high : power_low);
+        float sc[4 * kSubs];
+#pragma unroll
+        for (int j = 0; j < 4 * kSubs; ++j) sc[j] = s4[j / 4][j % 4];
         if (!full) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                unmapped |= no_page[half] && key0 + 16 * half < n && key0 + 16 * half + 16 > lo;
+            for (int sub = 0; sub < kSubs; ++sub) {
+                unmapped |= no_page[sub] && key0 + 16 * sub < n && key0 + 16 * sub + 16 > lo;
                 unsigned hidden = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int key = key0 + 16 * half + 4 * g + i;
-                    if (no_page[half] || key < lo || key >= n) sc[4 * half + i] = -INFINITY, hidden |= 0xffu << (8 * i);
+                    const int key = key0 + 16 * sub + 4 * g + i;
+                    if (no_page[sub] || key < lo || key >= n) sc[4 * sub + i] = -INFINITY, hidden |= 0xffu << (8 * i);
                 }
                 // what lies in places out of sight may be anything: a power of one makes it a number
 #pragma unroll
-                for (int s = 0; s < kVLoads; ++s) r.v_power[half][s] = (r.v_power[half][s] & ~hidden) | (0x7f7f7f7fu & hidden);
+                for (int s = 0; s < kVLoads; ++s) r.v_power[sub][s] = (r.v_power[sub][s] & ~hidden) | (0x7f7f7f7fu & hidden);
             }
         }
         float top = sc[0];
 #pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, sc[j]);
+        for (int j = 1; j < 4 * kSubs; ++j) top = fmaxf(top, sc[j]);
+        top *= to_log2;
         if (__any(top > m_ref + kRaise)) {                        // -inf + 8 is -inf: the first scores always raise
             top = max_lanes<16>(top);
             top = max_lanes<32>(top);
@@ -394,49 +400,53 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
 #pragma unroll
                 for (int v = 0; v < 4; ++v) acc[j][v] *= keep;
         }
-        const float shift = m_ref == -INFINITY ? 0.f : m_ref;
-        bf16x8 pt;
+        const float shift = m_ref == -INFINITY ? 0.f : -m_ref;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) pt[j] = static_cast<__bf16>(__builtin_amdgcn_exp2f(sc[j] - shift));
-        {
-            const uint4 packed = __builtin_bit_cast(uint4, pt);
-            const unsigned pairs[4] = {packed.x, packed.y, packed.z, packed.w};
+        for (int two = 0; two < kSubs / 2; ++two) {               // 32 keys of the second product
+            bf16x8 pt;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pairs[i]), __builtin_bit_cast(bf16x2, 0x3f803f80u), l_run, false);
-        }
-        // ---- values: the lane's elements of its eight tokens, two elements at a time from every token, then by element
+            for (int j = 0; j < 8; ++j) pt[j] = static_cast<__bf16>(__builtin_amdgcn_exp2f(fmaf(sc[8 * two + j], to_log2, shift)));
+            {
+                const uint4 packed = __builtin_bit_cast(uint4, pt);
+                const unsigned pairs[4] = {packed.x, packed.y, packed.z, packed.w};
 #pragma unroll
-        for (int s = 0; s < kVLoads; ++s) {
-            unsigned words[8];
-            float power[8];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const unsigned w[4] = {r.v[half][s].x, r.v[half][s].y, r.v[half][s].z, r.v[half][s].w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    words[4 * half + i] = kD <= 64 ? w[i] >> (16 * (c & 1)) : w[i];
-                    power[4 * half + i] = power_of(r.v_power[half][s] >> (8 * i) & 255u);
-                }
+                for (int i = 0; i < 4; ++i)
+                    l_run = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pairs[i]), __builtin_bit_cast(bf16x2, 0x3f803f80u), l_run, false);
             }
-            auto pair = [&](auto index) {
-                constexpr int i = decltype(index)::value;
-                unsigned two[8];
+            // ---- values: the lane's elements of its eight tokens, two elements at a time from every token, then by element
 #pragma unroll
-                for (int k = 0; k < 8; ++k) two[k] = two_bf16<i>(words[k], power[k]);
-                uint4 even, odd;
-                even.x = __builtin_amdgcn_perm(two[1], two[0], 0x05040100u), odd.x = __builtin_amdgcn_perm(two[1], two[0], 0x07060302u);
-                even.y = __builtin_amdgcn_perm(two[3], two[2], 0x05040100u), odd.y = __builtin_amdgcn_perm(two[3], two[2], 0x07060302u);
-                even.z = __builtin_amdgcn_perm(two[5], two[4], 0x05040100u), odd.z = __builtin_amdgcn_perm(two[5], two[4], 0x07060302u);
-                even.w = __builtin_amdgcn_perm(two[7], two[6], 0x05040100u), odd.w = __builtin_amdgcn_perm(two[7], two[6], 0x07060302u);
-                acc[8 * s + 2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), pt, acc[8 * s + 2 * i], 0, 0, 0);
-                acc[8 * s + 2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), pt, acc[8 * s + 2 * i + 1], 0, 0, 0);
-            };
-            pair(std::integral_constant<int, 0>{});
-            pair(std::integral_constant<int, 1>{});
-            if constexpr (kD > 64) {
-                pair(std::integral_constant<int, 2>{});
-                pair(std::integral_constant<int, 3>{});
+            for (int s = 0; s < kVLoads; ++s) {
+                unsigned words[8];
+                float power[8];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint4 raw = r.v[2 * two + half][s];
+                    const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        words[4 * half + i] = kD <= 64 ? w[i] >> (16 * (c & 1)) : w[i];
+                        power[4 * half + i] = power_of(r.v_power[2 * two + half][s] >> (8 * i) & 255u);
+                    }
+                }
+                auto pair = [&](auto index) {
+                    constexpr int i = decltype(index)::value;
+                    unsigned both[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) both[k] = two_bf16<i>(words[k], power[k]);
+                    uint4 even, odd;
+                    even.x = __builtin_amdgcn_perm(both[1], both[0], 0x05040100u), odd.x = __builtin_amdgcn_perm(both[1], both[0], 0x07060302u);
+                    even.y = __builtin_amdgcn_perm(both[3], both[2], 0x05040100u), odd.y = __builtin_amdgcn_perm(both[3], both[2], 0x07060302u);
+                    even.z = __builtin_amdgcn_perm(both[5], both[4], 0x05040100u), odd.z = __builtin_amdgcn_perm(both[5], both[4], 0x07060302u);
+                    even.w = __builtin_amdgcn_perm(both[7], both[6], 0x05040100u), odd.w = __builtin_amdgcn_perm(both[7], both[6], 0x07060302u);
+                    acc[8 * s + 2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), pt, acc[8 * s + 2 * i], 0, 0, 0);
+                    acc[8 * s + 2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), pt, acc[8 * s + 2 * i + 1], 0, 0, 0);
+                };
+                pair(std::integral_constant<int, 0>{});
+                pair(std::integral_constant<int, 1>{});
+                if constexpr (kD > 64) {
+                    pair(std::integral_constant<int, 2>{});
+                    pair(std::integral_constant<int, 3>{});
+                }
             }
         }
     };
