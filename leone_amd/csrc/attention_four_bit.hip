@@ -34,7 +34,6 @@
 
 namespace leone {
 
-
 // Query heads a workgroup of the decode kernel takes: a product has sixteen columns; wide heads' sums take the room of eight.
 __host__ __device__ constexpr int decode_columns(int dim) { return dim <= 128 ? 16 : 8; }
 
@@ -64,8 +63,9 @@ four_bit_attend_rows_kernel(const T* __restrict__ q, T* __restrict__ out, FourBi
     const int row = blockIdx.x, kvh = blockIdx.y / head_tiles, head0 = kvh * group + blockIdx.y % head_tiles * kRowsHeads;
     const int heads = min(kRowsHeads, (kvh + 1) * group - head0);
     const int entry = row_entry[row];
-    const int n = entry >= 0 && entry < entries ? positions[row] + 1 : 0;
-    const int lo = first_key(n - 1, window, 0);
+    const int all = entry >= 0 && entry < entries ? min(positions[row], kLastPosition) + 1 : 0;
+    const int lo = first_key(max(all - 1, 0), window, 0);
+    const int n = min(all, max_blocks * page_tokens);            // keys behind the block table's reach have no page
     const int* table = block_table + static_cast<long>(entry) * max_blocks;
     for (int i = threadIdx.x; i < kRowsHeads * kD; i += kRowsThreads) {
         const int h = i / kD, d = i % kD;
@@ -79,7 +79,7 @@ four_bit_attend_rows_kernel(const T* __restrict__ q, T* __restrict__ out, FourBi
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[h][i] = 0.f;
     }
-    bool unmapped = false;
+    bool unmapped = n < all;
     const int t_begin = lo / kRowsKeys, t_end = (n + kRowsKeys - 1) / kRowsKeys;
     const int share = (t_end - t_begin + splits - 1) / splits;
     const int my_begin = t_begin + static_cast<int>(blockIdx.z) * share, my_end = min(my_begin + share, t_end);
@@ -216,7 +216,7 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
     constexpr int kSteps = kD <= 128 ? 1 : kD / 128;              // of 128 elements
     constexpr int kParts = kD <= 64 ? 1 : 2;                      // products a step: heads of 64 hold both parts of a query in one
     constexpr int kVLoads = kD <= 128 ? 1 : kD / 128;             // eights a lane has of each of its tokens
-    constexpr int kDepth = kD <= 128 ? 2 : 2;
+    constexpr int kDepth = 2;
     constexpr int kOwn = kD / 16;                                 // elements a lane has of each of its tokens
     extern __shared__ float smem[];                               // [waves][columns][kD], then maxima and sums
 
@@ -230,10 +230,9 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
     const int kvh = blockIdx.y / col_tiles, col0 = (blockIdx.y - kvh * col_tiles) * kCols;
     const int cols = min(kCols, group - col0), split = blockIdx.z;
     const int entry = row_entry[row], pos = positions[row];
-    const int all = entry >= 0 && entry < entries ? pos + 1 : 0;
-    const int lo = first_key(all - 1, window, 0);
-    // keys behind the block table's reach have no page
-    const int n = all > 0 ? static_cast<int>(min(static_cast<long>(all), static_cast<long>(max_blocks) << page_shift)) : 0;
+    const int all = entry >= 0 && entry < entries ? min(pos, kLastPosition) + 1 : 0;
+    const int lo = first_key(max(all - 1, 0), window, 0);
+    const int n = min(all, max_blocks << page_shift);             // keys behind the block table's reach have no page
     const int* table = block_table + static_cast<long>(entry) * max_blocks;
     const int t_begin = lo / kTileKeys, t_end = (n + kTileKeys - 1) / kTileKeys;
     const int share = (t_end - t_begin + splits - 1) / splits;
@@ -527,8 +526,6 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
     }
 }
 
-
-
 // The merge of shares.  kGroup neighbouring lanes have a row and head, four elements each; between them they hold the shares' maxima and
 // sums and hand the weights round, four shares' sums on their way at a time.
 constexpr int kMergeThreads = 256;
@@ -537,7 +534,7 @@ constexpr int kMergeAhead = 4;
 template <int kGroup, typename T>
 __global__ void __launch_bounds__(kMergeThreads)
 four_bit_merge_kernel(const float* __restrict__ part_acc, const float* __restrict__ part_ml, T* __restrict__ out, long items, int q_heads, int dim,
-                      int splits, const int* __restrict__ tiles) {
+                      int splits, const int* __restrict__ tiles, int limit) {
     constexpr int kEach = kShares / kGroup;                      // shares whose weights a lane holds
     const int lane = threadIdx.x % kGroup;
     long item = (static_cast<long>(blockIdx.x) * kMergeThreads + threadIdx.x) / kGroup;
@@ -547,7 +544,7 @@ four_bit_merge_kernel(const float* __restrict__ part_acc, const float* __restric
         const long place = item / q_heads;
         const int* tile = tiles + 3 * (place / kTileRows);
         const int r = static_cast<int>(place % kTileRows);
-        exists &= r < tile[2];
+        exists &= r < tile[2] && tile[1] >= 0 && tile[1] < limit - r;
         item = exists ? (static_cast<long>(tile[1]) + r) * q_heads + item % q_heads : 0;
     }
     const float* ml = part_ml + 2 * item * splits;
@@ -592,10 +589,10 @@ four_bit_merge_kernel(const float* __restrict__ part_acc, const float* __restric
 
 template <typename T>
 static void launch_merge(const float* part_acc, const float* part_ml, T* out, long items, int q_heads, int dim, int splits, const int* tiles,
-                         hipStream_t stream) {
+                         int limit, hipStream_t stream) {
 #define LEONE_MERGE(GROUP)                                                                                                                    \
     four_bit_merge_kernel<GROUP, T><<<ceil_div(items * GROUP, kMergeThreads), kMergeThreads, 0, stream>>>(part_acc, part_ml, out, items, q_heads, \
-                                                                                                         dim, splits, tiles)
+                                                                                                         dim, splits, tiles, limit)
     if (dim <= 64) LEONE_MERGE(16);
     else if (dim <= 128) LEONE_MERGE(32);
     else LEONE_MERGE(64);
@@ -603,10 +600,10 @@ static void launch_merge(const float* part_acc, const float* part_ml, T* out, lo
 }
 
 void merge_four_bit_shares(const float* part_acc, const float* part_ml, void* out, int dtype, long rows, int q_heads, int dim, int splits,
-                           const int* tiles, hipStream_t stream) {
+                           const int* tiles, int limit, hipStream_t stream) {
     const long items = rows * q_heads;
-    if (dtype == kF32) launch_merge(part_acc, part_ml, static_cast<float*>(out), items, q_heads, dim, splits, tiles, stream);
-    else launch_merge(part_acc, part_ml, static_cast<bf16_t*>(out), items, q_heads, dim, splits, tiles, stream);
+    if (dtype == kF32) launch_merge(part_acc, part_ml, static_cast<float*>(out), items, q_heads, dim, splits, tiles, limit, stream);
+    else launch_merge(part_acc, part_ml, static_cast<bf16_t*>(out), items, q_heads, dim, splits, tiles, limit, stream);
 }
 
 }  // namespace leone
@@ -626,6 +623,7 @@ extern "C" int leone_four_bit_attend_rows(const void* q, void* out, int dtype, c
     LEONE_REQUIRE(dtype == kF32 || dtype == kBF16, "%s: unknown type", what);
     LEONE_REQUIRE(rows > 0 && entries > 0 && q_heads > 0 && q_heads % kv_heads == 0, "%s: %d rows, %d entries, %d query heads over %d kv heads", what, rows,
                   entries, q_heads, kv_heads);
+    LEONE_REQUIRE(scale > 0.f, "%s: the score scale must be positive", what);
     LEONE_REQUIRE(window >= 0 && splits >= 1 && splits <= kShares, "%s: window %d must not be negative, splits %d in 1..%d", what, window, splits, kShares);
     LEONE_REQUIRE(splits == 1 || (part_acc && part_ml && reinterpret_cast<uintptr_t>(part_acc) % 16 == 0), "%s: %d shares need the workspace", what, splits);
     const int group = q_heads / kv_heads;
@@ -650,7 +648,7 @@ extern "C" int leone_four_bit_attend_rows(const void* q, void* out, int dtype, c
 #undef LEONE_ROWS
     LEONE_LAUNCH_CHECK(what);
     if (splits > 1) {
-        merge_four_bit_shares(part_acc, part_ml, out, dtype, rows, q_heads, head_dim, splits, nullptr, stream);
+        merge_four_bit_shares(part_acc, part_ml, out, dtype, rows, q_heads, head_dim, splits, nullptr, rows, stream);
         LEONE_LAUNCH_CHECK("four_bit_merge");
     }
     return 0;
@@ -668,6 +666,7 @@ extern "C" int leone_four_bit_decode(const void* q, void* out, const void* k_cod
     LEONE_REQUIRE(page_tokens >= 16 && (page_tokens & (page_tokens - 1)) == 0, "%s: pages of a power of two tokens from 16 on, not %d", what, page_tokens);
     LEONE_REQUIRE(rows > 0 && entries > 0 && q_heads > 0 && q_heads % kv_heads == 0, "%s: %d rows, %d entries, %d query heads over %d kv heads", what, rows,
                   entries, q_heads, kv_heads);
+    LEONE_REQUIRE(scale > 0.f, "%s: the score scale must be positive", what);
     LEONE_REQUIRE(window >= 0 && splits >= 1 && splits <= kShares, "%s: window %d must not be negative, splits %d in 1..%d", what, window, splits, kShares);
     LEONE_REQUIRE(splits == 1 || (part_acc && part_ml && reinterpret_cast<uintptr_t>(part_acc) % 16 == 0), "%s: %d shares need the workspace", what, splits);
     LEONE_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 == 0, "%s: queries and results start at multiples of 16 bytes", what);
@@ -697,7 +696,7 @@ extern "C" int leone_four_bit_decode(const void* q, void* out, const void* k_cod
 #undef LEONE_DECODE_CALL
     LEONE_LAUNCH_CHECK(what);
     if (splits > 1) {
-        merge_four_bit_shares(part_acc, part_ml, out, kBF16, rows, q_heads, head_dim, splits, nullptr, stream);
+        merge_four_bit_shares(part_acc, part_ml, out, kBF16, rows, q_heads, head_dim, splits, nullptr, rows, stream);
         LEONE_LAUNCH_CHECK("four_bit_merge");
     }
     return 0;

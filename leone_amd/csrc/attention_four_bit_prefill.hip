@@ -63,7 +63,7 @@ struct PromptStage {
 template <int kD, bool kWide>
 __global__ void __launch_bounds__(kPromptThreads, 2)
 four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, FourBitPools pools, const int* __restrict__ positions,
-                        const int* __restrict__ tiles, int n_groups, const int* __restrict__ block_table, int max_blocks, int entries,
+                        const int* __restrict__ tiles, int n_groups, int rows, const int* __restrict__ block_table, int max_blocks, int entries,
                         int q_heads, int kv_heads, int page_shift, float to_log2, int window, int splits, float* __restrict__ part_acc,
                         float* __restrict__ part_ml) {
     constexpr int kBlocks = kD / kBlock;              // blocks of a vector
@@ -89,21 +89,24 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
     const int page_tokens = 1 << page_shift, page_mask = page_tokens - 1;
     const int* my_tile = tiles + 3 * (static_cast<long>(work.group) * kPromptWaves + wave);
     const int entry = tiles[3 * static_cast<long>(work.group) * kPromptWaves];
-    const int tile_row0 = my_tile[1], wave_rows = min(my_tile[2], kTileRows);
+    // (rows that are not there, or that the workspace has no room for, are no tile's)
+    const int tile_row0 = my_tile[1], wave_rows = tile_row0 < 0 ? 0 : min(min(my_tile[2], kTileRows), rows - tile_row0);
     const bool entry_ok = entry >= 0 && entry < entries;
-    const int p0 = wave_rows > 0 ? positions[tile_row0] : 0;     // a tile's rows stand at consecutive positions
+    const int p0 = wave_rows > 0 ? min(positions[tile_row0], kLastPosition) : 0;     // a tile's rows stand at consecutive positions
     const int p_last = p0 + wave_rows - 1;
-    const int key_hi = wave_rows > 0 && entry_ok ? p_last + 1 : 0;      // keys the wave may read: [key_lo, key_hi)
+    const int reach = max_blocks << page_shift;                  // keys behind it have no page
+    const int key_hi = wave_rows > 0 && entry_ok ? min(p_last + 1, reach) : 0;      // keys the wave may read: [key_lo, key_hi)
     const int key_lo = first_key(max(p0, 0), window, 0);
     const int full_hi = p0 + 1, full_lo = wave_rows > 0 ? first_key(p_last, window, 0) : 0;    // keys that every row of the wave sees
     if (lane == 0) {
-        wave_lo[wave] = key_hi > 0 ? key_lo : 0x7fffffff;
-        wave_hi[wave] = key_hi;
+        wave_lo[wave] = key_hi > key_lo ? key_lo : 0x7fffffff;
+        wave_hi[wave] = key_hi > key_lo ? key_hi : 0;
     }
     if (tid == 0) unmapped_seen = 0;
     if (tid < 3 * kBlocks) nan_keys[tid / kBlocks][tid % kBlocks] = 0;
     if (tid < 3) nan_seen[tid] = 0;
     __syncthreads();
+    if (wave_rows > 0 && entry_ok && p_last >= reach) unmapped_seen = 1;
     int group_lo = 0x7fffffff, group_hi = 0;
 #pragma unroll
     for (int w = 0; w < kPromptWaves; ++w) group_lo = min(group_lo, wave_lo[w]), group_hi = max(group_hi, wave_hi[w]);
@@ -426,7 +429,7 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
 using namespace leone;
 
 extern "C" int leone_four_bit_prefill(const void* q, void* out, const void* k_codes, const void* k_powers, const void* v_codes, const void* v_powers,
-                                      int pages, const int* positions, const int* tiles, int n_groups, const int* block_table, int max_blocks,
+                                      int pages, const int* positions, const int* tiles, int n_groups, int rows, const int* block_table, int max_blocks,
                                       int entries, int q_heads, int kv_heads, int head_dim, int page_tokens, float scale, int window, int splits,
                                       float* part_acc, float* part_ml, hipStream_t stream) {
     const char* what = "four_bit_prefill";
@@ -435,6 +438,8 @@ extern "C" int leone_four_bit_prefill(const void* q, void* out, const void* k_co
     LEONE_REQUIRE(q && out && positions && tiles && block_table, "%s: null pointer", what);
     LEONE_REQUIRE(head_dim == 64 || head_dim == 128, "%s: heads of 64 or 128 elements, not %d", what, head_dim);
     LEONE_REQUIRE(page_tokens >= 16 && (page_tokens & (page_tokens - 1)) == 0, "%s: pages of a power of two tokens from 16 on, not %d", what, page_tokens);
+    LEONE_REQUIRE(scale > 0.f, "%s: the score scale must be positive", what);
+    LEONE_REQUIRE(rows > 0, "%s: %d rows", what, rows);
     LEONE_REQUIRE(n_groups > 0 && entries > 0 && q_heads > 0 && q_heads % kv_heads == 0, "%s: %d tile groups, %d entries, %d query heads over %d kv heads",
                   what, n_groups, entries, q_heads, kv_heads);
     LEONE_REQUIRE(static_cast<long>(n_groups) * q_heads <= 0x7fffffffL / kTileRows, "%s: too many tile groups", what);
@@ -448,7 +453,7 @@ extern "C" int leone_four_bit_prefill(const void* q, void* out, const void* k_co
     const dim3 grid(n_groups * q_heads, splits);
 #define LEONE_PREFILL_CALL(D, WIDE)                                                                                                            \
     four_bit_prefill_kernel<D, WIDE><<<grid, kPromptThreads, 0, stream>>>(static_cast<const bf16_t*>(q), static_cast<bf16_t*>(out), pools,     \
-                                                                          positions, tiles, n_groups, block_table, max_blocks, entries, q_heads, \
+                                                                          positions, tiles, n_groups, rows, block_table, max_blocks, entries, q_heads, \
                                                                           kv_heads, page_shift, scale * kLog2e, window, splits, part_acc, part_ml)
 #define LEONE_PREFILL(D)                                             \
     do {                                                             \
@@ -461,7 +466,7 @@ extern "C" int leone_four_bit_prefill(const void* q, void* out, const void* k_co
 #undef LEONE_PREFILL_CALL
     LEONE_LAUNCH_CHECK(what);
     if (splits > 1) {
-        merge_four_bit_shares(part_acc, part_ml, out, kBF16, static_cast<long>(n_groups) * kPromptWaves * kTileRows, q_heads, head_dim, splits, tiles, stream);
+        merge_four_bit_shares(part_acc, part_ml, out, kBF16, static_cast<long>(n_groups) * kPromptWaves * kTileRows, q_heads, head_dim, splits, tiles, rows, stream);
         LEONE_LAUNCH_CHECK("four_bit_merge");
     }
     return 0;

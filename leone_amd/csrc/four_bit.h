@@ -20,6 +20,10 @@ namespace leone {
 
 constexpr int kBlock = 32;                         // elements that share a power of two
 constexpr int kNanPower = 255;
+// Tokens that a block table may reach, and the last position that is told from those behind it (all of them without a page): what is
+// computed from positions stays within 32 bits.
+constexpr int kReach = 1 << 30;
+constexpr int kLastPosition = kReach + (1 << 20);
 
 struct FourBitPools {
     uint8_t* k_codes;
@@ -69,6 +73,8 @@ inline int check_four_bit(const char* what, const FourBitPools& p, int kv_heads,
     LEONE_REQUIRE((reinterpret_cast<uintptr_t>(p.k_codes) | reinterpret_cast<uintptr_t>(p.k_powers) | reinterpret_cast<uintptr_t>(p.v_codes) |
                    reinterpret_cast<uintptr_t>(p.v_powers)) % 16 == 0, "%s: the pools start at multiples of 16 bytes", what);
     LEONE_REQUIRE(p.pages > 0 && kv_heads > 0 && max_blocks > 0, "%s: %d pages, %d kv heads, block tables of %d", what, p.pages, kv_heads, max_blocks);
+    LEONE_REQUIRE(static_cast<long>(max_blocks) * page_tokens <= kReach, "%s: block tables of %d pages of %d tokens reach further than 2^30 tokens", what,
+                  max_blocks, page_tokens);
     LEONE_REQUIRE(dim % kBlock == 0 && dim >= kBlock && dim <= 256, "%s: heads of %d elements; blocks of 32 need a multiple of 32 up to 256", what, dim);
     LEONE_REQUIRE(page_tokens % 8 == 0 && page_tokens >= 8 && page_tokens <= 4096, "%s: pages of %d tokens; a multiple of 8 up to 4,096 is needed", what, page_tokens);
     return 0;

@@ -56,10 +56,11 @@ inline FourBitPools read_pools(const void* k_codes, const void* k_powers, const 
 
 // Merges the shares of a (row, query head) in their order: sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), from part_acc [rows *
 // q_heads, splits, dim] and part_ml [rows * q_heads, splits, 2]; shares with a maximum of -inf count as nothing, a row with no other
-// gives zeros.  With a list of tiles (entry, first row, rows up to 32) the rows are theirs, n_tiles * 32 places of them.
+// gives zeros.  With a list of tiles (entry, first row, rows up to 32) `rows` is their number times 32 and the rows are theirs, as far as
+// they lie below `limit`.
 constexpr int kShares = kWave;                     // the most shares
 constexpr int kTileRows = 32;
 void merge_four_bit_shares(const float* part_acc, const float* part_ml, void* out, int dtype, long rows, int q_heads, int dim, int splits,
-                           const int* tiles, hipStream_t stream);
+                           const int* tiles, int limit, hipStream_t stream);
 
 }  // namespace leone

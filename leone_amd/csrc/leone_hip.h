@@ -594,9 +594,9 @@ int leone_four_bit_decode(const void* q, void* out, const void* k_codes, const v
                           float* part_acc, float* part_ml, hipStream_t stream);
 
 // leone_attention_prefill over such a cache: heads of 64 or 128 elements, pages of a power of two tokens from 16 on, up to 32 ranges.  Only the rows
-// that a tile names are written.
+// that a tile names, and that lie below `rows`, are written; the workspace has room for `rows` of them.
 int leone_four_bit_prefill(const void* q, void* out, const void* k_codes, const void* k_powers, const void* v_codes, const void* v_powers,
-                           int pages, const int* positions, const int* tiles, int n_groups, const int* block_table, int max_blocks,
+                           int pages, const int* positions, const int* tiles, int n_groups, int rows, const int* block_table, int max_blocks,
                            int entries, int q_heads, int kv_heads, int head_dim, int page_tokens, float scale, int window, int splits,
                            float* part_acc, float* part_ml, hipStream_t stream);
 

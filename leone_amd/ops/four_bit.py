@@ -3,9 +3,9 @@
 A cached key or value vector is kept in blocks of 32 consecutive elements, each a number of the 4-bit floating type e2m1 times
 a power of two of the block's own (``csrc/four_bit.h`` says how they are chosen and laid out).  A cache is four byte tensors
 (``FourBitPools``); a token and kv head of ``dim`` elements take ``dim + dim / 16`` bytes, key and value together, against
-``4 * dim`` in bfloat16.  Queries, masks, block tables and results are those of the attention over a bfloat16 or float32 cache
-(``ops.attention_rows`` and its neighbours); a row that sees no key (position -1) gives zeros, a row in whose sight a place has no page
-gives NaN.
+``4 * dim`` in bfloat16.  A block table reaches up to 2^30 tokens.  Queries, masks, block tables and results are those of the attention
+over a bfloat16 or float32 cache (``ops.attention_rows`` and its neighbours); a row that sees no key (position -1) gives zeros, a row in
+whose sight a place has no page gives NaN.
 """
 from __future__ import annotations
 
@@ -17,6 +17,7 @@ from . import (F32, PREFILL_GROUP_TILES, KernelError, _CODES, _code, _dev, _rota
 
 BLOCK = 32                   # elements that share a power of two
 FOUR_BIT_MAX_DIM = 256
+MAX_SHARES = 64
 
 
 class FourBitPools(NamedTuple):
@@ -111,7 +112,7 @@ def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_heads: int, kv_heads: int, head
     k and v into the cache and returns q.  ``qkv`` is ``[rows, width]`` of q's type, or float32 (also as planes ``[p, rows, width]``
     whose sum is meant) with ``out_dtype`` naming the type of q.  Queries are rounded once, to that type; keys are computed in 64
     bits up to their codes.  Rows at a position below 0, and rows whose place has no page, write nothing; without ``write_cache`` (a run
-    that reads what another one of the layer's wrote) none does."""
+    that reads what another one of the layer's wrote) none does.  Of two rows at one place either may be kept, or parts of both."""
     what = "qk_norm_rope_write_4bit"
     planes = qkv.shape[0] if qkv.dim() == 3 else 1
     if qkv.dim() not in (2, 3) or qkv.shape[-1] != (q_heads + 2 * kv_heads) * head_dim or planes < 1:
@@ -172,6 +173,8 @@ def _shares_at(rows: int, q_heads: int, dim: int, splits: int, device) -> tuple:
     """(a tensor to hold on to, partial results of rows whose keys are shared out, their maxima and sums)."""
     if splits == 1:
         return None, 0, 0
+    if not 1 <= splits <= MAX_SHARES:
+        raise KernelError(f"a row's keys are cut into 1 to {MAX_SHARES} parts, not {splits}")
     shares = rows * q_heads * splits
     held = torch.empty((shares * (dim + 2),), dtype=torch.float32, device=device)
     at = held.data_ptr()
@@ -259,8 +262,8 @@ def attention_prefill_4bit(q: torch.Tensor, out: torch.Tensor, pools, positions:
                            q_heads: int, scale: float, window: int = 0, mean_keys: int = 1, splits: Optional[int] = None,
                            covered_rows: Optional[int] = None) -> torch.Tensor:
     """``attention_prefill`` over a cache of 4 bits an element (``four_bit_prefill_supported``): attention for the rows that ``tiles``
-    covers, into ``out``; other rows of ``out`` are left as they are.  ``tiles``, ``mean_keys`` and ``covered_rows`` as there.  A key in
-    sight of a group of tiles whose place has no page makes the group's rows NaN."""
+    covers, into ``out``; other rows of ``out``, and rows from ``covered_rows`` on, are left as they are.  ``tiles``, ``mean_keys`` and
+    ``covered_rows`` as there.  A key in sight of a group of tiles whose place has no page makes the group's rows NaN."""
     what = "attention_prefill_4bit"
     kv_heads, page_tokens, dim = _attention_shape(what, q, pools, q_heads, window)
     if not four_bit_prefill_supported(q.dtype, dim, page_tokens):
@@ -278,7 +281,7 @@ def attention_prefill_4bit(q: torch.Tensor, out: torch.Tensor, pools, positions:
     device = _current(what, q)
     held, part_acc, part_ml = _shares_at(covered, q_heads, dim, splits, q.device)
     args = (_at(what, "q", q, device, q.dtype, q.shape), _at(what, "out", out, device, q.dtype, q.shape), *_pools_at(what, pools, device),
-            _at(what, "positions", positions, device, torch.int32, (rows,)), _at(what, "tiles", tiles, device, torch.int32, tiles.shape), groups,
+            _at(what, "positions", positions, device, torch.int32, (rows,)), _at(what, "tiles", tiles, device, torch.int32, tiles.shape), groups, covered,
             _at(what, "block table", block_table, device, torch.int32, block_table.shape), block_table.shape[1], block_table.shape[0], q_heads,
             kv_heads, dim, page_tokens, scale, window, splits, part_acc, part_ml)
     if groups and covered:

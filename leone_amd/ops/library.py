@@ -162,7 +162,7 @@ _PROTOTYPES = {
                             c_int, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P],
     "leone_four_bit_rows": [P, P, P, P, c_int, P, P, P, c_int, c_int, P, P, c_int, c_int, c_int, c_int, P],
     "leone_four_bit_max_splits": [],
-    "leone_four_bit_prefill": [P, P, P, P, P, P, c_int, P, P, c_int, P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, P, P, P],
+    "leone_four_bit_prefill": [P, P, P, P, P, P, c_int, P, P, c_int, c_int, P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, P, P, P],
     "leone_four_bit_decode": [P, P, P, P, P, P, c_int, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, P, P, P],
     "leone_four_bit_attend_rows": [P, P, c_int, P, P, P, P, c_int, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
                                    P, P, P],

@@ -316,6 +316,138 @@ def test_portions_that_see_nan_or_no_page(splits, dim):
     assert torch.isnan(out[130:258]).all() and torch.isfinite(out[:130]).all()
 
 
+def test_a_run_recorded_and_replayed():
+    """Filling, single tokens and reading back as a step does them, recorded once: every replay, with other work and synchronizations
+    between, gives what the eager run gives; two recordings and an eager run do not share a workspace."""
+    gen = _generator(21)
+    lengths, heads, dim = [700, 65, 1, 333], 2, 128
+    pools, table, _ = _cache(gen, lengths, heads, dim, 64)
+    positions, entries = _rows([(n - 1, 1) for n in lengths])
+    angles = torch.outer(torch.arange(700, device=DEVICE).double(), 1e4 ** (-torch.arange(0, dim, 2, device=DEVICE).double() / dim))
+    cos, sin = angles.cos().float(), angles.sin().float()
+    gains = [torch.ones(dim, device=DEVICE)] * 2
+    projections = [_normal(gen, 4, 12 * dim).to(torch.bfloat16) for _ in range(3)]
+
+    def step(qkv, splits):
+        q = ops.qk_norm_rope_write_4bit(qkv, 8, heads, dim, *gains, 1e-6, cos, sin, positions, entries, table, pools)
+        out = ops.attention_decode_4bit(q, pools, positions, entries, table, 8, dim ** -0.5, splits=splits)
+        rows = ops.attention_rows_4bit(q, pools, positions, entries, table, 8, dim ** -0.5, splits=splits)
+        return (q, out, rows, *ops.cache_rows_4bit(pools, positions, entries, table))
+
+    recorded = []
+    stream = torch.cuda.Stream()
+    given = projections[0].clone()
+    with torch.cuda.stream(stream):
+        for splits in (1, 3):
+            step(given, splits)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                recorded.append((graph, splits, step(given, splits)))
+    for turn in range(4):
+        given.copy_(projections[turn % 3])
+        for graph, splits, got in recorded:
+            with torch.cuda.stream(stream):
+                stream.wait_stream(torch.cuda.default_stream())
+                graph.replay()
+            torch.cuda.synchronize()
+            want = step(given, splits)
+            _normal(gen, 1 << 18).sum().item()
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (turn, splits)
+
+
+def test_calls_on_two_streams_at_once():
+    gen = _generator(22)
+    cases = []
+    for i in range(2):
+        pools, table, _ = _cache(gen, [900, 400], 2, 128, 64)
+        positions, entries = _rows([(899, 1), (399, 1)])
+        q = _normal(gen, 2, 8 * 128).to(torch.bfloat16)
+        cases.append((q, pools, positions, entries, table, 8, 128 ** -0.5))
+    want = [ops.attention_decode_4bit(*c, splits=3) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(20):
+        for i, (c, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(ops.attention_decode_4bit(*c, splits=3))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for outs, w in zip(got, want) for o in outs)
+
+
+def test_queries_alone_and_rows_behind_the_covered_ones():
+    gen = _generator(23)
+    pools, table, _ = _cache(gen, [200], 2, 128, 64)
+    before = [p.clone() for p in pools]
+    positions, entries = _rows([(100, 100)])
+    qkv = _normal(gen, 100, 8 * 128).to(torch.bfloat16)
+    q = ops.qk_norm_rope_write_4bit(qkv, 4, 2, 128, None, None, 1e-6, None, None, positions, entries, table, pools, write_cache=False)
+    assert torch.equal(q, qkv[:, :512]) and all(torch.equal(a, b) for a, b in zip(pools, before))
+    # tiles that name more rows than are covered, or rows that are not there: nothing of theirs is written
+    tiles = torch.tensor([(0, 0, 32), (0, 32, 32), (0, 64, 32), (0, 96, 32), (0, -3, 8), (0, 5000, 32), (0, 0, 0), (0, 0, 0)], dtype=torch.int32, device=DEVICE)
+    for splits in (1, 2):
+        out = torch.full_like(q, 5.0)
+        ops.attention_prefill_4bit(q, out, pools, positions, tiles, table, 4, 128 ** -0.5, splits=splits, covered_rows=70)
+        whole = ops.attention_prefill_4bit(q, torch.empty_like(q), pools, positions, tiles[:4], table, 4, 128 ** -0.5, splits=splits)
+        assert torch.equal(out[:70], whole[:70]) and (out[70:] == 5.0).all()
+
+
+def test_long_tables_and_offsets_past_32_bits():
+    """A cache of more than 2^31 bytes of codes, its last pages read and written; pages far down a long table."""
+    heads, dim, page = 8, 128, 64
+    pages = (1 << 31) // (heads * page * dim // 2) + 40
+    pools = ops.four_bit_pools(pages, heads, dim, page, DEVICE)
+    gen = _generator(24)
+    n = 150
+    blocks = 3000
+    table = torch.full((1, blocks), -1, dtype=torch.int32, device=DEVICE)
+    first = (blocks - 3) * page
+    table[0, blocks - 3:] = torch.tensor([pages - 1, 3, pages - 20], dtype=torch.int32, device=DEVICE)
+    positions = torch.arange(first, first + n, dtype=torch.int32, device=DEVICE)
+    entries = torch.zeros_like(positions)
+    qkv = _normal(gen, n, 3 * heads * dim).to(torch.bfloat16)
+    q = ops.qk_norm_rope_write_4bit(qkv, heads, heads, dim, None, None, 1e-6, None, None, positions, entries, table, pools)
+    k, v = ops.cache_rows_4bit(pools, positions, entries, table)
+    x = qkv.double().reshape(n, 3 * heads, dim)
+    keys, values = quantised(x[:, heads:2 * heads]), quantised(x[:, 2 * heads:])
+    assert torch.equal(k.double().reshape(n, heads, dim), keys) and torch.equal(v.double().reshape(n, heads, dim), values)
+    window = 128                                              # within the mapped pages of the last rows
+    rows = slice(n - 20, n)
+    want = torch.stack([attended(q[i].reshape(heads, dim), torch.cat([keys[:i + 1]]), torch.cat([values[:i + 1]]), i, dim ** -0.5, window)[0]
+                        for i in range(n - 20, n)])
+    tiles = ops.prefill_tiles([(0, n - 20, 20)]).to(DEVICE)
+    for out in (ops.attention_decode_4bit(q[rows], pools, positions[rows], entries[rows], table, heads, dim ** -0.5, window),
+                ops.attention_rows_4bit(q[rows], pools, positions[rows], entries[rows], table, heads, dim ** -0.5, window),
+                ops.attention_prefill_4bit(q, torch.zeros_like(q), pools, positions, tiles, table, heads, dim ** -0.5, window)[rows]):
+        # weights rounded to 2^-8 and a result rounded once: values of size 1 to 3, sums of 128 of them
+        assert (out.double().reshape(20, heads, dim) - want).abs().max() <= 2.0 ** -8 * (4 + 4 * 3 / 128 ** 0.5)
+
+
+@pytest.mark.parametrize("window", [0, 16, 1 << 30])
+@pytest.mark.parametrize("splits", [1, 4])
+def test_positions_behind_the_table(window, splits):
+    """Places that the block table does not reach have no page, up to the largest position there is: NaN, and nothing is written."""
+    gen = _generator(25)
+    pools, table, _ = _cache(gen, [256], 2, 128, 64)
+    reach = table.shape[1] * 64
+    before = [p.clone() for p in pools]
+    last = 2 ** 31 - 1
+    positions = torch.tensor([last, reach, 100, last - 1, last - 40, -1, -last - 1, 1 << 30], dtype=torch.int32, device=DEVICE)
+    entries = torch.zeros_like(positions)
+    qkv = _normal(gen, 8, 8 * 128).to(torch.bfloat16)
+    q = ops.qk_norm_rope_write_4bit(qkv, 4, 2, 128, None, None, 1e-6, None, None, torch.where(positions == 100, -1, positions), entries, table, pools)
+    assert all(torch.equal(a, b) for a, b in zip(pools, before))
+    args = (pools, positions, entries, table, 4, 128 ** -0.5, window)
+    nan = torch.tensor([True, True, False, True, True, False, False, True], device=DEVICE)
+    tiles = torch.tensor([(0, r, 1) for r in range(8)] + [(0, 0, 0)] * 24, dtype=torch.int32, device=DEVICE)
+    tiles = tiles.reshape(4, 8, 3).transpose(0, 1).reshape(32, 3).contiguous()        # each row a group of its own
+    for out in (ops.attention_decode_4bit(q, *args, splits=splits), ops.attention_rows_4bit(q, *args, splits=splits),
+                ops.attention_prefill_4bit(q, torch.full_like(q, 5.0), pools, positions, tiles, table, 4, 128 ** -0.5, window, splits=splits)):
+        assert torch.equal(out.isnan().all(dim=1), nan) and not out[~nan].isnan().any()
+        assert (out[5:7] == 0).all() and (out[2] != 0).any()
+
+
 def test_refusals():
     gen = _generator(2)
     pools, table, _ = _cache(gen, [64], 2, 64, 64)
@@ -323,8 +455,9 @@ def test_refusals():
     q = torch.zeros(1, 4 * 64, dtype=torch.bfloat16, device=DEVICE)
     good = dict(q=q, pools=pools, positions=positions, row_entry=entries, block_table=table, q_heads=4, scale=0.125)
     ops.attention_rows_4bit(**good)
+    far = torch.zeros((1, (1 << 30) // pools[0].shape[3] + 1), dtype=torch.int32, device=DEVICE)
     for change in (dict(q=q.half()), dict(q_heads=3), dict(positions=positions.long()), dict(pools=pools[:3]), dict(window=-1), dict(splits=0),
-                   dict(splits=65), dict(block_table=table[0]), dict(row_entry=entries.repeat(2)), dict(q=q.cpu()), dict(positions=positions.cpu()),
+                   dict(scale=0.0), dict(scale=-1.0), dict(row_entry=None), dict(splits=10 ** 9), dict(block_table=far), dict(splits=65), dict(block_table=table[0]), dict(row_entry=entries.repeat(2)), dict(q=q.cpu()), dict(positions=positions.cpu()),
                    dict(pools=(pools[0], pools[1], pools[2], pools[1])), dict(pools=tuple(p.int() for p in pools)), dict(q=q.repeat(2, 1)[:, ::2])):
         with pytest.raises(KernelError):
             ops.attention_rows_4bit(**{**good, **change})
