@@ -38,13 +38,14 @@ def _engine(folder, dtype_name, **options):
     return Engine(model, max_requests=4, cache_bits=4, **options)
 
 
-def _plain(config, weights, tokens, kept):
-    """The plain implementation whose attention reads ``kept(layer, keys, values)``; logits, and the layers' own keys and values."""
+def _plain(config, weights, tokens, kept, windows=None):
+    """The plain implementation whose attention reads ``kept(layer, keys, values)``; logits, and the layers' own keys and values.
+    ``windows``: of layers that have one."""
     exact, seen = qwen3_plain.causal_attention, []
 
     def attention(q, k, v, window=None):
         seen.append((k, v))
-        return exact(q, *kept(len(seen) - 1, k, v), window)
+        return exact(q, *kept(len(seen) - 1, k, v), (windows or {}).get(len(seen) - 1, window))
 
     try:
         qwen3_plain.causal_attention = attention
@@ -154,6 +155,31 @@ def test_forks_share_pages_and_requests_are_cut_back(cases):
     engine.truncate("a", 32)                                   # (within a page that is shared it cannot be cut)
     out = engine.step([StepEntry("a", toks[32:], [len(toks) - 33])]).logits
     assert (out - whole).abs().max() <= tolerance("float32")
+
+
+@pytest.mark.parametrize("schedule", list(SCHEDULES))
+def test_windows_and_attention_as_a_branch(cases, schedule):
+    """A layer that sees the last 20 tokens (its pages behind them are given back) and one whose attention is a branch of a mixer of
+    several, which keeps its cache under a name."""
+    import dataclasses
+    from leone_amd.architectures import config_from_dict, model_spec_for
+    from leone_amd.engine.engine import Engine
+    from leone_amd.parts.base import PartSpec
+    from leone_amd.parts.model import DecoderModel
+    from leone_amd.weights import loader
+    folder, config, weights, requests = cases("B", "float32")
+    spec = model_spec_for(config_from_dict(config))
+    first, second = (dict(layer.params) for layer in spec.layers[:2])
+    first["mixer"] = PartSpec("gqa_attention", {**first["mixer"].params, "window": 20})
+    second["mixer"] = PartSpec("parallel", {"hidden": config["hidden_size"], "eps": 1e-6, "weights": {"only": 1.0},
+                                            "branches": {"only": PartSpec("gqa_attention", {**second["mixer"].params, "float_output": True})}})
+    spec = dataclasses.replace(spec, layers=[PartSpec("prenorm", first), PartSpec("prenorm", second), *spec.layers[2:]])
+    model = DecoderModel(spec, torch.float32, "cuda:0")
+    model.bind(loader.load_from_dir(folder, model.tensor_specs(), torch.float32, torch.device("cuda:0"), ignore=spec.ignore_tensors))
+    expected = {rid: _plain(config, weights, toks, lambda layer, k, v: (quantised(k), quantised(v)), {0: 20})[0] for rid, toks in requests.items()}
+    engine = Engine(model, max_requests=4, cache_bits=4, max_tokens=512, page_tokens=16, poison_freed=True)
+    steps = list(SCHEDULES[schedule](requests))
+    compare(steps, run_steps(engine, steps), expected, tolerance("float32"), schedule)
 
 
 def test_models_and_sizes_that_do_not_fit_are_refused(cases, tmp_path):
