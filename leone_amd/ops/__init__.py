@@ -52,14 +52,14 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _held = threading.local()                # .stream inside ``one_stream``: the handle that was current when it began
 
 
-def _stream() -> int:
-    """The current stream's handle.  Asked for before every launch, so the short way is taken where this
+def _stream(device: Optional[int] = None) -> int:
+    """The current stream's handle (``device``: the current device, of a caller that has it at hand).  Asked for before every launch, so the short way is taken where this
     torch has it (a tenth of the time of building a Stream object); within ``one_stream`` it was asked for once."""
     held = getattr(_held, "stream", None)
     if held is not None:
         return held
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(torch.cuda.current_device() if device is None else device)
     return torch.cuda.current_stream().cuda_stream
 
 

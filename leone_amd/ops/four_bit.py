@@ -52,10 +52,10 @@ def four_bit_dims(pools) -> tuple:
         pages, kv_heads, blocks, page_tokens, block_bytes = k_codes.shape
     except (ValueError, AttributeError, TypeError):
         raise KernelError("a cache of 4 bits an element is four tensors: key codes, key powers, value codes, value powers") from None
-    dim = blocks * BLOCK
-    if (block_bytes != 16 or k_powers.shape != (pages, kv_heads, page_tokens, blocks)
-            or v_codes.shape != (pages, kv_heads, page_tokens // 4, dim // 8, 4, 4)
-            or v_powers.shape != (pages, kv_heads, page_tokens // 4, blocks, 4) or not four_bit_supported(dim, page_tokens)):
+    dim, runs = blocks * BLOCK, page_tokens // 4
+    if (block_bytes != 16 or k_powers.shape != (pages, kv_heads, page_tokens, blocks) or v_codes.shape != (pages, kv_heads, runs, 4 * blocks, 4, 4)
+            or v_powers.shape != (pages, kv_heads, runs, blocks, 4) or page_tokens % 8 or not 8 <= page_tokens <= 4096
+            or not BLOCK <= dim <= FOUR_BIT_MAX_DIM):
         raise KernelError(f"pools of shapes {tuple(tuple(p.shape) for p in pools)} are no cache of 4 bits an element")
     return pages, kv_heads, page_tokens, dim
 
@@ -78,6 +78,20 @@ def _at(what: str, name: str, t: torch.Tensor, device: int, dtype: torch.dtype, 
         return t.data_ptr()
     _dev(t, f"{what}: {name}", dtype, shape)
     raise KernelError(f"{what}: {name} is on {t.device}, the others on cuda:{device}; one device is needed")
+
+
+def _pair_at(what: str, name: str, a: Optional[torch.Tensor], b: Optional[torch.Tensor], device: int, dtype: Optional[torch.dtype],
+             shape: Optional[tuple]) -> tuple:
+    """The addresses of two operands that come together or not at all, of one type and shape (None: the first one's)."""
+    if a is None or b is None:
+        if a is not b:
+            raise KernelError(f"{what}: one {name} of two")
+        return 0, 0
+    dtype, shape = dtype or a.dtype, shape or a.shape
+    if (a.dtype is b.dtype is dtype and a.shape == shape and b.shape == shape and a.get_device() == b.get_device() == device and a.is_contiguous()
+            and b.is_contiguous()):
+        return a.data_ptr(), b.data_ptr()
+    return _at(what, f"first {name}", a, device, dtype, shape), _at(what, f"second {name}", b, device, dtype, shape)
 
 
 def _pools_at(what: str, pools, device: int) -> tuple:
@@ -128,19 +142,15 @@ def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_heads: int, kv_heads: int, head
     if (q_gain is None) != (k_gain is None) or (q_gain is not None and k_gain.dtype != q_gain.dtype):
         raise KernelError(f"{what}: q and k gains must come together in one type")
     if out is None:
-        out = torch.empty((rows, q_heads * head_dim), dtype=kind, device=qkv.device)
+        out = qkv.new_empty((rows, q_heads * head_dim), dtype=kind)
     device = _current(what, qkv)
-    float32 = torch.float32
     args = (_at(what, "qkv", qkv, device, qkv.dtype, qkv.shape), _CODES[qkv.dtype], planes, rows * width, width,
             _at(what, "q out", out, device, kind, (rows, q_heads * head_dim)), _CODES[kind], *_pools_at(what, pools, device),
-            0 if q_gain is None else _at(what, "q gain", q_gain, device, q_gain.dtype, (head_dim,)),
-            0 if k_gain is None else _at(what, "k gain", k_gain, device, k_gain.dtype, (head_dim,)),
-            F32 if q_gain is None else _code(q_gain, "qk_norm_rope_write_4bit: gain"), eps,
-            0 if cos is None else _at(what, "cos", cos, device, float32, cos.shape), 0 if sin is None else _at(what, "sin", sin, device, float32, sin.shape),
-            table_positions, rotary_dim, pairing_code, *_rows_at(what, device, rows, positions, row_entry, block_table), rows, q_heads, kv_heads,
+            *_pair_at(what, "gain", q_gain, k_gain, device, None, (head_dim,)), F32 if q_gain is None else _code(q_gain, "qk_norm_rope_write_4bit: gain"),
+            eps, *_pair_at(what, "table", cos, sin, device, torch.float32, None), table_positions, rotary_dim, pairing_code, *_rows_at(what, device, rows, positions, row_entry, block_table), rows, q_heads, kv_heads,
             head_dim, page_tokens, 1 if write_cache else 0)
     if rows:
-        call("leone_four_bit_fill", *args, _stream())
+        call("leone_four_bit_fill", *args, _stream(device))
     return out
 
 
@@ -151,12 +161,12 @@ def cache_rows_4bit(pools, positions: torch.Tensor, row_entry: torch.Tensor, blo
     pages, kv_heads, page_tokens, dim = four_bit_dims(pools)
     device = _current(what, positions)
     rows = positions.shape[0]
-    k = torch.empty((rows, kv_heads * dim), dtype=torch.bfloat16, device=positions.device)
+    k = positions.new_empty((rows, kv_heads * dim), dtype=torch.bfloat16)
     v = torch.empty_like(k)
     args = (*_pools_at(what, pools, device), *_rows_at(what, device, rows, positions, row_entry, block_table), k.data_ptr(), v.data_ptr(), rows,
             kv_heads, dim, page_tokens)
     if rows:
-        call("leone_four_bit_rows", *args, _stream())
+        call("leone_four_bit_rows", *args, _stream(device))
     return k, v
 
 
@@ -176,7 +186,7 @@ def _shares_at(rows: int, q_heads: int, dim: int, splits: int, device) -> tuple:
     if not 1 <= splits <= MAX_SHARES:
         raise KernelError(f"a row's keys are cut into 1 to {MAX_SHARES} parts, not {splits}")
     shares = rows * q_heads * splits
-    held = torch.empty((shares * (dim + 2),), dtype=torch.float32, device=device)
+    held = torch.empty(shares * (dim + 2), dtype=torch.float32, device=device)
     at = held.data_ptr()
     return held, at, at + 4 * shares * dim
 
@@ -209,7 +219,7 @@ def attention_rows_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_ent
             *_pools_at(what, pools, device), *_rows_at(what, device, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, dim, page_tokens,
             scale, window, splits, part_acc, part_ml)
     if rows:
-        call("leone_four_bit_attend_rows", *args, _stream())
+        call("leone_four_bit_attend_rows", *args, _stream(device))
     return out
 
 
@@ -249,7 +259,7 @@ def attention_decode_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_e
             *_rows_at(what, device, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, dim, page_tokens, scale, window, splits,
             part_acc, part_ml)
     if rows:
-        call("leone_four_bit_decode", *args, _stream())
+        call("leone_four_bit_decode", *args, _stream(device))
     return out
 
 
@@ -285,5 +295,5 @@ def attention_prefill_4bit(q: torch.Tensor, out: torch.Tensor, pools, positions:
             _at(what, "block table", block_table, device, torch.int32, block_table.shape), block_table.shape[1], block_table.shape[0], q_heads,
             kv_heads, dim, page_tokens, scale, window, splits, part_acc, part_ml)
     if groups and covered:
-        call("leone_four_bit_prefill", *args, _stream())
+        call("leone_four_bit_prefill", *args, _stream(device))
     return out

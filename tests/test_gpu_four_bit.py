@@ -466,7 +466,7 @@ def test_refusals():
     ops.qk_norm_rope_write_4bit(**fill)
     ones = torch.ones(64, device=DEVICE)
     angles = torch.zeros(64, 33, device=DEVICE)
-    for change in (dict(q_heads=3), dict(kv_heads=1), dict(q_gain=ones), dict(q_gain=ones, k_gain=ones.bfloat16()), dict(cos=angles, sin=angles),
+    for change in (dict(q_heads=3), dict(kv_heads=1), dict(q_gain=ones), dict(q_gain=ones, k_gain=ones.bfloat16()), dict(cos=angles, sin=angles), dict(sin=angles[:, :32].contiguous()), dict(k_gain=ones),
                    dict(pairing="odd"), dict(cos=angles[:, :32].contiguous()), dict(out_dtype=torch.float32), dict(out_dtype=torch.float16),
                    dict(row_entry=None and entries, positions=positions[:0]), dict(q_gain=ones[:32], k_gain=ones[:32])):
         with pytest.raises(KernelError):
