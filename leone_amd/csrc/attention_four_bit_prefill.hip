@@ -6,10 +6,17 @@
 // into the first product as they are:
 // v_mfma_scale_f32_32x32x64_f8f6f4, 4-bit keys with their powers against queries in two 8-bit parts (see attention_four_bit.hip).  It takes as
 // long as the bfloat16 product of the same size would, but a wave reads a quarter of the bytes from shared memory, which four waves
-// with 32 rows each read all keys from.  (By loads that write to shared memory themselves the compiler waits for the next stage's
-// before it reads this one's: 322 us where this takes 2xx.)  Values are unpacked once for the four waves: a thread has four tokens of eight elements
+// with 32 rows each read all keys from.  Values are unpacked once for the four waves: a thread has four tokens of eight elements
 // in flight while a stage is worked on, turns them into runs of eight tokens of one element and leaves them in shared memory for
-// the next, in bfloat16, where v_mfma_f32_32x32x16_bf16 takes them.
+// the next, in bfloat16, where v_mfma_f32_32x32x16_bf16 takes them.  Both come by way of registers, asked for two stages ahead: loads
+// that write to shared memory themselves are waited for before it is read again.
+//
+// 2,048 rows behind 8,192 tokens, 32 heads of 128 over 8: 294 us, 1,050 TFLOP/s of the exact work (a product of two 8,192-square bfloat16
+// matrices reaches 1,200 by the vendor library, the bfloat16 prompt kernel 927 here); 128 rows behind 30,720, 64 heads: 147 us in 8 ranges
+// and their merge, 8 of them.  A pass of 32 keys is 512 cycles of the matrix cores and 560 of vector instructions (a weight is an
+// exponential, a value a conversion and a permutation), and the two waves of a SIMD overlap them in part: the matrix cores are busy 42 %
+// of the time, the vector units 46 %.  Forcing the overlap does not pay: two heads a workgroup, four waves a phase behind the other four
+// with a barrier a phase 382 us; a pass's products asked for before the last one's weights 321; two heads a wave 481.
 //
 // Operand layouts (lane l, j = l % 32, h = l / 32): 4-bit operand: row j, elements 32 h .. + 31; 8-bit operand: column j, elements 16 h ..
 // + 15 and 32 + 16 h .. + 15; a lane's power belongs to elements 32 h .. + 31 of its row or column; result: column j, rows
@@ -82,7 +89,7 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
     const int j = lane & 31, h = lane >> 5;
     // Two workgroups share a unit: the second half of those that fit at a time goes first where both have something to issue, so that one
-    // multiplies while the other makes weights instead of both doing the same (2,048 rows behind 8,192 tokens 322 us without, 308 with).
+    // multiplies while the other makes weights instead of both doing the same (worth a twentieth).
     if ((blockIdx.x + blockIdx.y * gridDim.x) / kPromptUnits % 2) __builtin_amdgcn_s_setprio(1);
     const PrefillWork work = prefill_work(static_cast<int>(blockIdx.x), q_heads, n_groups);
     const int head = work.head, kvh = head / (q_heads / kv_heads);
@@ -158,8 +165,8 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
             }
         }
 
-        // ---- bringing a stage by way of registers, a stage ahead: a thread's unit of keys is block `k_block` of key k_key, its values eight `v_eight` of the four tokens
-        // from v_key; a wave's lanes also hold the powers of the keys that they multiply.
+        // ---- bringing a stage by way of registers: a thread's unit of keys is block `k_block` of key k_key, its values eight `v_eight`
+        // of the four tokens from v_key; a wave's lanes also hold the powers of the keys that they multiply.
         const int* table = block_table + static_cast<long>(entry) * max_blocks;
         const long code_bytes = four_bit_codes(page_tokens, kD), power_bytes = four_bit_powers(page_tokens, kD);
         const bool brings = kKeyUnits == kPromptThreads || tid < kKeyUnits;
