@@ -11,11 +11,11 @@
 // the next, in bfloat16, where v_mfma_f32_32x32x16_bf16 takes them.  Both come by way of registers, asked for two stages ahead: loads
 // that write to shared memory themselves are waited for before it is read again.
 //
-// 2,048 rows behind 8,192 tokens, 32 heads of 128 over 8: 294 us, 1,050 TFLOP/s of the exact work (a product of two 8,192-square bfloat16
-// matrices reaches 1,200 by the vendor library, the bfloat16 prompt kernel 927 here); 128 rows behind 30,720, 64 heads: 147 us in 8 ranges
+// 2,048 rows behind 8,192 tokens, 32 heads of 128 over 8: 283 us, 1,095 TFLOP/s of the exact work (a product of two 8,192-square bfloat16
+// matrices reaches 1,200 by the vendor library, the bfloat16 prompt kernel 927 here); 128 rows behind 30,720, 64 heads: 143 us in 8 ranges
 // and their merge, 8 of them.  A pass of 32 keys is 512 cycles of the matrix cores and 560 of vector instructions (a weight is an
-// exponential, a value a conversion and a permutation), and the two waves of a SIMD overlap them in part: the matrix cores are busy 42 %
-// of the time, the vector units 46 %.  Forcing the overlap does not pay: two heads a workgroup, four waves a phase behind the other four
+// exponential, a value a conversion and a permutation), and the two waves of a SIMD overlap them in part: the matrix cores are busy 44 %
+// of the time, the vector units 47 %.  Forcing the overlap does not pay: two heads a workgroup, four waves a phase behind the other four
 // with a barrier a phase 382 us; a pass's products asked for before the last one's weights 321; two heads a wave 481.
 //
 // Operand layouts (lane l, j = l % 32, h = l / 32): 4-bit operand: row j, elements 32 h .. + 31; 8-bit operand: column j, elements 16 h ..
@@ -48,7 +48,6 @@ constexpr int kPromptThreads = kPromptWaves * kWave;
 constexpr int kStageKeys = 64;
 constexpr int kPassKeys = 32;
 constexpr int kMaxRanges = 32;
-constexpr int kPromptUnits = 256;                     // compute units: workgroups that get one of their own
 
 // Row of a pass's first product <-> key of the pass.
 __device__ inline int pass_key(int x) { return (x & 0x13) | ((x & 4) << 1) | ((x & 8) >> 1); }
@@ -88,9 +87,6 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
 
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
     const int j = lane & 31, h = lane >> 5;
-    // Two workgroups share a unit: the second half of those that fit at a time goes first where both have something to issue, so that one
-    // multiplies while the other makes weights instead of both doing the same (worth a twentieth).
-    if ((blockIdx.x + blockIdx.y * gridDim.x) / kPromptUnits % 2) __builtin_amdgcn_s_setprio(1);
     const PrefillWork work = prefill_work(static_cast<int>(blockIdx.x), q_heads, n_groups);
     const int head = work.head, kvh = head / (q_heads / kv_heads);
     const int page_tokens = 1 << page_shift, page_mask = page_tokens - 1;
@@ -240,12 +236,13 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
         auto deposit = [&](int note, PromptStage<kD>* to) {
             if (brings) {
                 to->keys[tid] = k_codes;
-                unsigned nan_tokens = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) nan_tokens |= (v_powers >> (8 * i) & 255u) == 255u ? 1u << i : 0u;
+                const unsigned clear = ~v_powers;                // a byte of 255 is one of zero here
                 unsigned words[4] = {v_codes.x, v_codes.y, v_codes.z, v_codes.w};
                 unsigned powers = v_powers;
-                if (nan_tokens != 0) {
+                if (((clear - 0x01010101u) & v_powers & 0x80808080u) != 0) {
+                    unsigned nan_tokens = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) nan_tokens |= (v_powers >> (8 * i) & 255u) == 255u ? 1u << i : 0u;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (nan_tokens >> i & 1u) words[i] = 0, powers = (powers & ~(0xffu << (8 * i))) | (0x7fu << (8 * i));
@@ -280,6 +277,10 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
             intx8 key[kSteps];
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) key[s] = low_half(from->keys[(half * kBlocks + 2 * s + h) * 32 + j]);
+            // Two waves share a SIMD and do best when one multiplies while the other makes weights or unpacks: who is further on in a pass goes first,
+            // and what belongs to no pass waits (2,048 rows behind 8,192 tokens 306 us without, 294 with every second 256 workgroups ahead, 283 so;
+            // whole passes ahead of the rest 285, products ahead of weights 307).
+            __builtin_amdgcn_s_setprio(1);
             sc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(key[0], query[0][0], sc, 4, 0, 0, powers, 0, power_high);
             sc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(key[0], query[0][1], sc, 4, 0, 0, powers, 0, power_low);
             if constexpr (kSteps > 1) {
@@ -299,6 +300,7 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
                     sc[v] = key_at <= row_pos && key_at >= row_lo && key_at >= group_lo && key_at < group_hi ? sc[v] : -INFINITY;
                 }
             }
+            __builtin_amdgcn_s_setprio(2);
             float top = sc[0];
 #pragma unroll
             for (int v = 1; v < 16; ++v) top = fmaxf(top, sc[v]);
@@ -329,6 +331,7 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
             for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                 for (int dt = 0; dt < kDT; ++dt) acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xv[ks][dt], pt[ks], acc[dt], 0, 0, 0);
+            __builtin_amdgcn_s_setprio(0);
         };
         // Which of a block's elements register v of tile dt holds: row r = 8 (v / 4) + 4 h + v % 4 of the tile is place 32 dt + r.
         auto block_of = [&](int dt, int v) {
