@@ -11,7 +11,7 @@
 // the next, in bfloat16, where v_mfma_f32_32x32x16_bf16 takes them.  Both come by way of registers, asked for two stages ahead: loads
 // that write to shared memory themselves are waited for before it is read again.
 //
-// 2,048 rows behind 8,192 tokens, 32 heads of 128 over 8: 283 us, 1,095 TFLOP/s of the exact work (a product of two 8,192-square bfloat16
+// 2,048 rows behind 8,192 tokens, 32 heads of 128 over 8: 281 us, 1,100 TFLOP/s of the exact work (a product of two 8,192-square bfloat16
 // matrices reaches 1,200 by the vendor library, the bfloat16 prompt kernel 927 here); 128 rows behind 30,720, 64 heads: 143 us in 8 ranges
 // and their merge, 8 of them.  A pass of 32 keys is 512 cycles of the matrix cores and 560 of vector instructions (a weight is an
 // exponential, a value a conversion and a permutation), and the two waves of a SIMD overlap them in part: the matrix cores are busy 44 %
@@ -269,23 +269,20 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
         };
 
         // ---- one pass of a wave: 32 keys against its 32 rows
-        auto pass = [&](const PromptStage<kD>* from, int key0, int half, bool full) {
+        auto pass = [&](const PromptStage<kD>* from, const uint4 key[kSteps], int key0, int half, bool full) {
             floatx16 sc;
 #pragma unroll
             for (int v = 0; v < 16; ++v) sc[v] = 0.f;
             const int powers = static_cast<int>(k_powers[half] >> (8 * h));
-            intx8 key[kSteps];
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) key[s] = low_half(from->keys[(half * kBlocks + 2 * s + h) * 32 + j]);
-            // Two waves share a SIMD and do best when one multiplies while the other makes weights or unpacks: who is further on in a pass goes first,
-            // and what belongs to no pass waits (2,048 rows behind 8,192 tokens 306 us without, 294 with every second 256 workgroups ahead, 283 so;
-            // whole passes ahead of the rest 285, products ahead of weights 307).
+            // Two waves share a SIMD and do best when one multiplies while the other makes weights or unpacks: who is further on in a
+            // pass goes first, and what belongs to no pass waits (2,048 rows behind 8,192 tokens 306 us without, 294 with every second 256
+            // workgroups ahead, 283 so; whole passes ahead of the rest 285, products ahead of weights 307).
             __builtin_amdgcn_s_setprio(1);
-            sc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(key[0], query[0][0], sc, 4, 0, 0, powers, 0, power_high);
-            sc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(key[0], query[0][1], sc, 4, 0, 0, powers, 0, power_low);
+            sc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(low_half(key[0]), query[0][0], sc, 4, 0, 0, powers, 0, power_high);
+            sc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(low_half(key[0]), query[0][1], sc, 4, 0, 0, powers, 0, power_low);
             if constexpr (kSteps > 1) {
-                sc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(key[kSteps - 1], query[kSteps - 1][0], sc, 4, 0, 2, powers, 0, power_high);
-                sc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(key[kSteps - 1], query[kSteps - 1][1], sc, 4, 0, 2, powers, 0, power_low);
+                sc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(low_half(key[kSteps - 1]), query[kSteps - 1][0], sc, 4, 0, 2, powers, 0, power_high);
+                sc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(low_half(key[kSteps - 1]), query[kSteps - 1][1], sc, 4, 0, 2, powers, 0, power_low);
             }
             bf16x8 xv[2][kDT];
 #pragma unroll
@@ -372,11 +369,16 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
         // `note`, `next_note`, `old_note`: whose NaN keys are read, written and cleared in this round
         auto round = [&](const PromptStage<kD>* __restrict__ reading, PromptStage<kD>* __restrict__ writing, int t, int note, int next_note, int old_note) {
             const int any_nan = nan_seen[note];                   // (asked for with the keys, used behind them)
+            uint4 keys[2][kSteps];                               // (of both passes: the second does not wait for its own)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) keys[half][s] = reading->keys[(half * kBlocks + 2 * s + h) * 32 + j];
             const bool plain = t >= plain_begin && t < plain_end;    // nothing to mask: most stages of a long context
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int key0 = t * kStageKeys + half * kPassKeys;
-                if (plain || (key0 < key_hi && key0 + kPassKeys > key_lo)) pass(reading, key0, half, plain);
+                if (plain || (key0 < key_hi && key0 + kPassKeys > key_lo)) pass(reading, keys[half], key0, half, plain);
                 if (half == 0) {
                     if (t + 1 < t_end) deposit(next_note, writing);
                     k_powers_ready[0] = k_powers_next[0], k_powers_ready[1] = k_powers_next[1];
