@@ -618,8 +618,6 @@ void merge_four_bit_shares(const float* part_acc, const float* part_ml, void* ou
 
 using namespace leone;
 
-extern "C" int leone_four_bit_max_splits() { return kShares; }
-
 extern "C" int leone_four_bit_attend_rows(const void* q, void* out, int dtype, const void* k_codes, const void* k_powers, const void* v_codes,
                                           const void* v_powers, int pages, const int* positions, const int* row_entry, const int* block_table,
                                           int max_blocks, int entries, int rows, int q_heads, int kv_heads, int head_dim, int page_tokens,
@@ -634,6 +632,7 @@ extern "C" int leone_four_bit_attend_rows(const void* q, void* out, int dtype, c
     LEONE_REQUIRE(scale > 0.f, "%s: the score scale must be positive", what);
     LEONE_REQUIRE(window >= 0 && splits >= 1 && splits <= kShares, "%s: window %d must not be negative, splits %d in 1..%d", what, window, splits, kShares);
     LEONE_REQUIRE(splits == 1 || (part_acc && part_ml && reinterpret_cast<uintptr_t>(part_acc) % 16 == 0), "%s: %d shares need the workspace", what, splits);
+    LEONE_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 == 0, "%s: queries and results start at multiples of 16 bytes", what);
     const int group = q_heads / kv_heads;
     const long tiles = static_cast<long>(kv_heads) * ((group + kRowsHeads - 1) / kRowsHeads);
     LEONE_REQUIRE(tiles <= 65535, "%s: too many heads for one launch", what);

@@ -578,10 +578,9 @@ int leone_four_bit_rows(const void* k_codes, const void* k_powers, const void* v
                         const int* positions, const int* row_entry, const int* block_table, int max_blocks, int entries, void* k_out,
                         void* v_out, int rows, int kv_heads, int head_dim, int page_tokens, hipStream_t stream);
 
-// Attention of each row over its request's cached keys (the last `window` of them; 0: all), any shape and type.  The keys of a row
-// are cut into `splits` parts (at most leone_four_bit_max_splits()); more than one need part_acc (rows * q_heads * splits * head_dim
-// floats) and part_ml (rows * q_heads * splits * 2).
-int leone_four_bit_max_splits();
+// Attention of each row over its request's cached keys (the last `window` of them; 0: all), any shape and type.  q and out start at
+// multiples of 16 bytes.  The keys of a row are cut into `splits` parts, up to 64; more than one need part_acc (rows * q_heads * splits *
+// head_dim floats) and part_ml (rows * q_heads * splits * 2).
 int leone_four_bit_attend_rows(const void* q, void* out, int dtype, const void* k_codes, const void* k_powers, const void* v_codes,
                                const void* v_powers, int pages, const int* positions, const int* row_entry, const int* block_table,
                                int max_blocks, int entries, int rows, int q_heads, int kv_heads, int head_dim, int page_tokens, float scale,

@@ -161,7 +161,6 @@ _PROTOTYPES = {
     "leone_four_bit_fill": [P, c_int, c_int, ctypes.c_long, ctypes.c_long, P, c_int, P, P, P, P, c_int, P, P, c_int, c_float, P, P, c_int, c_int,
                             c_int, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P],
     "leone_four_bit_rows": [P, P, P, P, c_int, P, P, P, c_int, c_int, P, P, c_int, c_int, c_int, c_int, P],
-    "leone_four_bit_max_splits": [],
     "leone_four_bit_prefill": [P, P, P, P, P, P, c_int, P, P, c_int, c_int, P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, P, P, P],
     "leone_four_bit_decode": [P, P, P, P, P, P, c_int, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, P, P, P],
     "leone_four_bit_attend_rows": [P, P, c_int, P, P, P, P, c_int, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,

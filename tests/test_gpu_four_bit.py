@@ -461,6 +461,17 @@ def test_refusals():
                    dict(pools=(pools[0], pools[1], pools[2], pools[1])), dict(pools=tuple(p.int() for p in pools)), dict(q=q.repeat(2, 1)[:, ::2])):
         with pytest.raises(KernelError):
             ops.attention_rows_4bit(**{**good, **change})
+    # contiguous, but not where runs of eight elements begin
+    apart = torch.zeros(8 * 64 + 1, dtype=torch.bfloat16, device=DEVICE)[1:]
+    tiles = torch.zeros(4, 3, dtype=torch.int32, device=DEVICE)
+    for change in (dict(q=apart[:256].view(1, 256)), dict(out=apart[:256].view(1, 256))):
+        for attend in (ops.attention_rows_4bit, ops.attention_decode_4bit):
+            with pytest.raises(KernelError, match="16 bytes"):
+                attend(**{**good, **change})
+        with pytest.raises(KernelError, match="16 bytes"):
+            ops.attention_prefill_4bit(change.get("q", q), change.get("out", torch.zeros_like(q)), pools, positions, tiles, table, 4, 0.125)
+    with pytest.raises(KernelError, match="16 bytes"):
+        ops.qk_norm_rope_write_4bit(apart.view(1, 512), 4, 2, 64, None, None, 1e-6, None, None, positions, entries, table, pools)
     fill = dict(qkv=torch.zeros(1, 8 * 64, dtype=torch.bfloat16, device=DEVICE), q_heads=4, kv_heads=2, head_dim=64, q_gain=None, k_gain=None, eps=1e-6,
                 cos=None, sin=None, positions=positions, row_entry=entries, block_table=table, pools=pools)
     ops.qk_norm_rope_write_4bit(**fill)
