@@ -14,7 +14,7 @@
 // 2,048 rows behind 8,192 tokens, 32 heads of 128 over 8: 281 us, 1,100 TFLOP/s of the exact work (a product of two 8,192-square bfloat16
 // matrices reaches 1,200 by the vendor library, the bfloat16 prompt kernel 927 here); 128 rows behind 30,720, 64 heads: 143 us in 8 ranges
 // and their merge, 8 of them.  A pass of 32 keys is 512 cycles of the matrix cores and 560 of vector instructions (a weight is an
-// exponential, a value a conversion and a permutation), and the two waves of a SIMD overlap them in part: the matrix cores are busy 44 %
+// exponential, a value a conversion and a permutation), and the two waves of a SIMD overlap them in part: the matrix cores are busy 45 %
 // of the time, the vector units 47 %.  Forcing the overlap does not pay: two heads a workgroup, four waves a phase behind the other four
 // with a barrier a phase 382 us; a pass's products asked for before the last one's weights 321; two heads a wave 481.
 //
@@ -366,7 +366,7 @@ four_bit_prefill_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, 
         fetch(min(t_begin + 1, t_end - 1), ahead);
         ahead = find(min(t_begin + 2, t_end - 1));
         shared_barrier();
-        // `note`, `next_note`, `old_note`: whose NaN keys are read, written and cleared in this round
+        // `note`, `next_note`, `old_note`: whose NaN keys are read, written and cleared while stage t is worked on
         auto round = [&](const PromptStage<kD>* __restrict__ reading, PromptStage<kD>* __restrict__ writing, int t, int note, int next_note, int old_note) {
             const int any_nan = nan_seen[note];                   // (asked for with the keys, used behind them)
             uint4 keys[2][kSteps];                               // (of both passes: the second does not wait for its own)
