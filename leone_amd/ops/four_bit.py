@@ -192,10 +192,11 @@ def _shares_at(rows: int, q_heads: int, dim: int, splits: int, device) -> tuple:
 
 
 def four_bit_row_splits(blocks: int, keys: int, units: int = 256) -> int:
-    """How many workgroups share a row's keys in ``attention_rows_4bit``, where ``blocks`` workgroups would have them all: as many as
-    leave none of the chip's units idle, but no more than give each of their four waves 64 keys (4 rows of 501 to 777 keys, 16 blocks:
-    21 us with 3, where some waves have two tiles, 14.1 with 4, 14.4 with 16)."""
-    return max(1, min(units // max(1, blocks), -(-keys // 256), 64))
+    """How many workgroups share a row's keys in ``attention_rows_4bit``, where ``blocks`` workgroups would have them all: four
+    workgroups for each of the chip's units, as many as fit one, but no more than give each of their four waves 64 keys.  us, by splits: 64
+    blocks of 8,176 keys 261 (1), 77 (4), 48 (8), 39 (16), 41 (32); 8 of them 63 (4), 24 (16), 19 (32); 256 of 2,000 74 (1), 37 (4), 38 (8),
+    56 (16); 512 of 4,000 169 (1), 116 (2), 111 (4), 206 (32); 16 of 501 to 777 21 (3: some waves have two tiles), 14.1 (4), 14.4 (16)."""
+    return max(1, min(4 * units // max(1, blocks), -(-keys // 256), MAX_SHARES))
 
 
 def attention_rows_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_entry: torch.Tensor, block_table: torch.Tensor, q_heads: int,
