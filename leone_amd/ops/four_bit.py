@@ -15,6 +15,9 @@ import torch
 
 from . import (F32, PREFILL_GROUP_TILES, KernelError, _CODES, _code, _dev, _rotation_shape, _stream, call, choose_prefill_splits, compute_units)
 
+# (a tensor on a GPU is there: nothing has to be initialised)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
 BLOCK = 32                   # elements that share a power of two
 FOUR_BIT_MAX_DIM = 256
 MAX_SHARES = 64
@@ -67,7 +70,7 @@ def _current(what: str, t: torch.Tensor) -> int:
     device = t.get_device()
     if device < 0:
         raise KernelError(f"{what}: tensor is on {t.device}; the kernels run on the GPU only")
-    if device != torch.cuda.current_device():
+    if device != _current_device():
         raise KernelError(f"{what}: tensors on {t.device}, which is not the current device")
     return device
 
@@ -141,11 +144,14 @@ def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_heads: int, kv_heads: int, head
     table_positions, rotary_dim, pairing_code = _rotation_shape(what, head_dim, cos, sin, pairing)
     if (q_gain is None) != (k_gain is None) or (q_gain is not None and k_gain.dtype != q_gain.dtype):
         raise KernelError(f"{what}: q and k gains must come together in one type")
+    device = _current(what, qkv)
     if out is None:
         out = qkv.new_empty((rows, q_heads * head_dim), dtype=kind)
-    device = _current(what, qkv)
+        out_at = out.data_ptr()
+    else:
+        out_at = _at(what, "q out", out, device, kind, (rows, q_heads * head_dim))
     args = (_at(what, "qkv", qkv, device, qkv.dtype, qkv.shape), _CODES[qkv.dtype], planes, rows * width, width,
-            _at(what, "q out", out, device, kind, (rows, q_heads * head_dim)), _CODES[kind], *_pools_at(what, pools, device),
+            out_at, _CODES[kind], *_pools_at(what, pools, device),
             *_pair_at(what, "gain", q_gain, k_gain, device, None, (head_dim,)), F32 if q_gain is None else _code(q_gain, "qk_norm_rope_write_4bit: gain"),
             eps, *_pair_at(what, "table", cos, sin, device, torch.float32, None), table_positions, rotary_dim, pairing_code, *_rows_at(what, device, rows, positions, row_entry, block_table), rows, q_heads, kv_heads,
             head_dim, page_tokens, 1 if write_cache else 0)
@@ -177,6 +183,14 @@ def _attention_shape(what: str, q: torch.Tensor, pools, q_heads: int, window: in
     if window < 0:
         raise KernelError(f"{what}: window {window} must not be negative")
     return kv_heads, page_tokens, dim
+
+
+def _out_at(what: str, q: torch.Tensor, out: Optional[torch.Tensor], device: int) -> tuple:
+    """(the results' tensor, its address); what is made here need not be asked."""
+    if out is None:
+        out = torch.empty_like(q)
+        return out, out.data_ptr()
+    return out, _at(what, "out", out, device, q.dtype, q.shape)
 
 
 def _shares_at(rows: int, q_heads: int, dim: int, splits: int, device) -> tuple:
@@ -212,11 +226,10 @@ def attention_rows_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_ent
         keys = max_context or block_table.shape[-1] * page_tokens
         keys = min(keys, window) if window else keys
         splits = four_bit_row_splits(rows * kv_heads * (-(-(q_heads // kv_heads) // 4)), keys, compute_units(q.device))
-    if out is None:
-        out = torch.empty_like(q)
     device = _current(what, q)
+    out, out_at = _out_at(what, q, out, device)
     held, part_acc, part_ml = _shares_at(rows, q_heads, dim, splits, q.device)
-    args = (_at(what, "q", q, device, q.dtype, q.shape), _at(what, "out", out, device, q.dtype, q.shape), _code(q, what),
+    args = (_at(what, "q", q, device, q.dtype, q.shape), out_at, _code(q, what),
             *_pools_at(what, pools, device), *_rows_at(what, device, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, dim, page_tokens,
             scale, window, splits, part_acc, part_ml)
     if rows:
@@ -252,11 +265,10 @@ def attention_decode_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_e
         keys = max_context or block_table.shape[-1] * page_tokens
         splits = four_bit_decode_splits(rows * kv_heads * -(-group // (16 if dim <= 128 else 8)), min(keys, window) if window else keys,
                                         compute_units(q.device))
-    if out is None:
-        out = torch.empty_like(q)
     device = _current(what, q)
+    out, out_at = _out_at(what, q, out, device)
     held, part_acc, part_ml = _shares_at(rows, q_heads, dim, splits, q.device)
-    args = (_at(what, "q", q, device, q.dtype, q.shape), _at(what, "out", out, device, q.dtype, q.shape), *_pools_at(what, pools, device),
+    args = (_at(what, "q", q, device, q.dtype, q.shape), out_at, *_pools_at(what, pools, device),
             *_rows_at(what, device, rows, positions, row_entry, block_table), rows, q_heads, kv_heads, dim, page_tokens, scale, window, splits,
             part_acc, part_ml)
     if rows:
