@@ -12,7 +12,7 @@
 // that write to shared memory themselves are waited for before it is read again.
 //
 // 2,048 rows behind 8,192 tokens, 32 heads of 128 over 8: 281 us, 1,100 TFLOP/s of the exact work (a product of two 8,192-square bfloat16
-// matrices reaches 1,200 by the vendor library, the bfloat16 prompt kernel 927 here); 128 rows behind 30,720, 64 heads: 143 us in 8 ranges
+// matrices reaches 1,200 by the vendor library, the bfloat16 prompt kernel 927 here); 128 rows behind 30,720, 64 heads: 131 to 143 us in 8 ranges
 // and their merge, 8 of them.  A pass of 32 keys is 512 cycles of the matrix cores and 560 of vector instructions (a weight is an
 // exponential, a value a conversion and a permutation), and the two waves of a SIMD overlap them in part: the matrix cores are busy 45 %
 // of the time, the vector units 47 %.  Forcing the overlap does not pay: two heads a workgroup, four waves a phase behind the other four
