@@ -194,7 +194,7 @@ four_bit_attend_rows_kernel(const T* __restrict__ q, T* __restrict__ out, FourBi
 #pragma unroll
         for (int w = 0; w < kRowsWaves; ++w) {
             const float by = part_m[w][h] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(part_m[w][h] - top);
-            if (by > 0.f) num += part[w][h][d] * by;
+            num += part[w][h][d] * by;                          // (a NaN value stays one however little it weighs)
             den += part_l[w][h] * by;
         }
         const long row_head = static_cast<long>(row) * q_heads + head0 + h;
@@ -538,6 +538,7 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
 // sums and hand the weights round, four shares' sums on their way at a time.
 constexpr int kMergeThreads = 256;
 constexpr int kMergeAhead = 4;
+constexpr float kNotWritten = -1.f;                              // in a weight's place: a share of no keys, whose sums may be anything
 
 template <int kGroup, typename T>
 __global__ void __launch_bounds__(kMergeThreads)
@@ -566,7 +567,7 @@ four_bit_merge_kernel(const float* __restrict__ part_acc, const float* __restric
     top = join_span<kGroup>(top, [](float a, float b) { return fmaxf(a, b); });
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-        const float w = m[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[k] - top);
+        const float w = m[k] == -INFINITY ? kNotWritten : __builtin_amdgcn_exp2f(m[k] - top);
         den += m[k] == -INFINITY ? 0.f : by[k] * w;
         by[k] = w;
     }
@@ -582,10 +583,10 @@ four_bit_merge_kernel(const float* __restrict__ part_acc, const float* __restric
             for (int i = 0; i < kMergeAhead; ++i)                // (a share behind the last is the last again and weighs nothing)
                 x[i] = *reinterpret_cast<const floatx4*>(from + static_cast<long>(min(s0 + i, splits - 1)) * dim);
 #pragma unroll
-            for (int i = 0; i < kMergeAhead; ++i) {
-                const float w = s0 + i < splits ? __shfl(by[k], (s0 + i) % kGroup, kGroup) : 0.f;
+            for (int i = 0; i < kMergeAhead; ++i) {              // (a weight that underflows is no reason: a NaN value stays one)
+                const float w = s0 + i < splits ? __shfl(by[k], (s0 + i) % kGroup, kGroup) : kNotWritten;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) num[e] = w > 0.f ? fmaf(x[i][e], w, num[e]) : num[e];   // (an empty share's sums were never written)
+                for (int e = 0; e < 4; ++e) num[e] = w == kNotWritten ? num[e] : fmaf(x[i][e], w, num[e]);
             }
         }
     }
