@@ -38,18 +38,18 @@ def prefill_flops(c, tokens: int, start: int = 0) -> float:
     return gemm + attention
 
 
-def cache_bytes_per_token(model) -> int:
-    """Bytes of keys and values one cached token takes over all cache slots of the model."""
+def cache_bytes_per_token(model, cache_bits: Optional[int] = None) -> int:
+    """Bytes of keys and values one cached token takes over all cache slots of the model (``cache_bits`` as for the engine)."""
     from .api import cache_bytes_per_token as per_token
-    return per_token(model)
+    return per_token(model, cache_bits)
 
 
-def decode_bytes(model, batch: int, context: float) -> float:
+def decode_bytes(model, batch: int, context: float, cache_bits: Optional[int] = None) -> float:
     """Bytes one decode step has to read: every weight it uses once (the model's own accounting), the rows
     of the stream, and the cache of the live requests."""
     size = 2 if str(model.dtype).endswith("bfloat16") else 4
     return (model.decode_step_weight_bytes(rows=batch) + batch * model.spec.hidden_size * size
-            + batch * context * cache_bytes_per_token(model))
+            + batch * context * cache_bytes_per_token(model, cache_bits))
 
 
 def measure_peaks(device: str = "cuda:0", megabytes: int = 1024, repeats: int = 5) -> dict:
@@ -96,17 +96,31 @@ def measure_peaks(device: str = "cuda:0", megabytes: int = 1024, repeats: int = 
 
 
 def fill_cache(engine, batch: int, tokens: int, seed: int = 0):
-    """Live requests with `tokens` positions each, their pages holding random keys and values (the
-    timed steps read them; what they hold does not change the work)."""
+    """Live requests with `tokens` positions each, their pages holding random keys and values: the timed steps
+    read them, and what they hold decides how often a softmax raises its reference and what power the chip draws."""
     import torch
+    from . import ops
     gen = torch.Generator(device=engine.device)
     gen.manual_seed(seed)
-    for k_pool, v_pool in ([] if getattr(engine, "_bench_filled", False) else engine.pools.kv.values()):
-        for pool in (k_pool, v_pool):
-            flat = pool.view(-1)
-            for at in range(0, flat.numel(), 1 << 28):
-                part = flat[at:at + (1 << 28)]
-                part.copy_(torch.randn(part.numel(), generator=gen, device=engine.device, dtype=torch.float32) * 0.5)
+
+    def fill(pool, fresh):
+        flat = pool.view(-1)
+        for at in range(0, flat.numel(), 1 << 28):
+            part = flat[at:at + (1 << 28)]
+            part.copy_(fresh(part.numel()))
+
+    def numbers(count):
+        return torch.randn(count, generator=gen, device=engine.device, dtype=torch.float32) * 0.5
+
+    for storage in ([] if getattr(engine, "_bench_filled", False) else engine.pools.paged.values()):
+        if isinstance(storage, ops.FourBitPools):
+            # any codes (their root mean square is 2.93 units) in units of 1/8 and 1/4: numbers of about the size of the others
+            for name, pool in zip(storage._fields, storage):
+                low, high = (124, 126) if name.endswith("powers") else (0, 256)
+                fill(pool, lambda count: torch.randint(low, high, (count,), generator=gen, device=engine.device, dtype=torch.uint8))
+        else:
+            for pool in storage:
+                fill(pool, numbers)
     engine._bench_filled = True
     for b in range(batch):
         engine.admit(("bench", b))
@@ -215,7 +229,7 @@ def time_generate(engine, batch: int, prompt_tokens: int, new_tokens: int, seed:
             "prefill_tok_s": generator.stats.prefill_rate, "wall_s": time.perf_counter() - total_started}
 
 
-def kernel_table(profiled, model, batch: int, context: float) -> dict:
+def kernel_table(profiled, model, batch: int, context: float, cache_bits: Optional[int] = None) -> dict:
     """Per operation of a decode step: microseconds a step and, where the operation streams something, the
     GB/s it reached (products: their weight bytes; attention: the cache of the live requests)."""
     steps = max(profiled.steps, 1)
@@ -228,7 +242,7 @@ def kernel_table(profiled, model, batch: int, context: float) -> dict:
                       "gbs": round(rows * columns * size * timing.calls / timing.seconds / 1e9, 1)}
     if "attention" in table:
         seconds = profiled.seconds_by_operation["attention"] / steps
-        table["attention"]["gbs"] = round(batch * context * cache_bytes_per_token(model) / seconds / 1e9, 1)
+        table["attention"]["gbs"] = round(batch * context * cache_bytes_per_token(model, cache_bits) / seconds / 1e9, 1)
     return table
 
 
@@ -583,6 +597,8 @@ def main(argv: Optional[List[str]] = None) -> int:
     parser.add_argument("--no-prefill", action="store_true")
     parser.add_argument("--no-kernels", action="store_true", help="skip the per-operation table of the decode step")
     parser.add_argument("--no-peaks", action="store_true", help="skip the measurement of this GPU's own peaks")
+    parser.add_argument("--cache-bits", type=int, choices=[4], default=None,
+                        help="keep keys and values in 4 bits an element (Engine(cache_bits=4)); not the headline figure")
     parser.add_argument("--no-streamed-weights", action="store_true",
                         help="keep no second copy of the matrices in the decode kernels' order")
     parser.add_argument("--tuned-products", action="store_true",
@@ -626,7 +642,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     # the cache takes requests of the context asked for and, for the prompt's figure, one of PREFILL_TOKENS
     engine = Engine(model, num_pages=pages, page_tokens=page_tokens, max_requests=largest + 1,
                     max_context=args.context if args.no_prefill else max(args.context, PREFILL_TOKENS),
-                    streamed_weights=False if args.no_streamed_weights else None)
+                    streamed_weights=False if args.no_streamed_weights else None, cache_bits=args.cache_bits)
 
     peaks = None if args.no_peaks else measure_peaks()
     profile_steps = 0 if args.no_kernels else 4
@@ -635,7 +651,7 @@ def main(argv: Optional[List[str]] = None) -> int:
     elapsed, mean_context = timed[0], timed[1]
     ms_per_step = elapsed / args.steps * 1e3
     value = args.batch * args.steps / elapsed
-    step_bytes = decode_bytes(model, args.batch, mean_context)
+    step_bytes = decode_bytes(model, args.batch, mean_context, args.cache_bits)
     achieved = step_bytes / (elapsed / args.steps) / 1e9
     record = {
         "metric": f"decode tok/s (Qwen3-{args.shape.upper()} shape)", "value": round(value, 2), "unit": "tok/s", "n_gpus": 1,
@@ -656,12 +672,15 @@ def main(argv: Optional[List[str]] = None) -> int:
     weights = model.weight_accounting(rows=args.batch)
     record["bytes"] = {"weights_resident": weights["tensor_bytes"], "weights_a_step": sum(weights["decode"].values()),
                        "weights_second_copy": weights["streamed_copy_bytes"],
-                       "cache_a_token": cache_bytes_per_token(model), "a_step": int(step_bytes)}
+                       "cache_a_token": cache_bytes_per_token(model, args.cache_bits), "a_step": int(step_bytes)}
+    if args.cache_bits is not None:
+        record["bytes"]["cache_bits"] = args.cache_bits
     if peaks is not None:
         record["peaks_measured"] = peaks
         record["roofline"]["frac_of_measured"] = round(achieved / peaks["hbm_read_gbs"], 4)
     if profile_steps:
-        record["kernels"] = kernel_table(timed[2], model, args.batch, start + args.warmup + args.steps + 2)
+        record["kernels"] = kernel_table(timed[2], model, args.batch, start + args.warmup + args.steps + 2,
+                                         args.cache_bits)
     if not args.no_prefill:
         # on request the vendor library's products of the prompt run with the fastest of the library's algorithms,
         # found by timing them now on this model's matrices (Engine.tune_products)
@@ -707,7 +726,8 @@ def main(argv: Optional[List[str]] = None) -> int:
         torch.cuda.empty_cache()
         long_context, long_batch = 32768, 8
         engine = Engine(model, num_pages=long_batch * (long_context // page_tokens + 1), page_tokens=page_tokens,
-                        max_requests=long_batch, streamed_weights=False if args.no_streamed_weights else None)
+                        max_requests=long_batch, streamed_weights=False if args.no_streamed_weights else None,
+                        cache_bits=args.cache_bits)
         assert engine.max_context == config.max_position_embeddings
         for batch in (1, long_batch):
             e, _ = time_decode(engine, batch, long_context - 40, 24, 8)
