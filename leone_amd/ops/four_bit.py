@@ -77,6 +77,8 @@ def _current(what: str, t: torch.Tensor) -> int:
 
 def _at(what: str, name: str, t: torch.Tensor, device: int, dtype: torch.dtype, shape: tuple) -> int:
     """The address of an operand that is as it has to be."""
+    if t is None:
+        raise KernelError(f"{what}: {name} is needed")
     if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
         return t.data_ptr()
     _dev(t, f"{what}: {name}", dtype, shape)
@@ -165,6 +167,8 @@ def cache_rows_4bit(pools, positions: torch.Tensor, row_entry: torch.Tensor, blo
     times its power is a bfloat16 as it is).  Rows without a page give NaN."""
     what = "cache_rows_4bit"
     pages, kv_heads, page_tokens, dim = four_bit_dims(pools)
+    if positions is None:
+        raise KernelError(f"{what}: positions are needed")
     device = _current(what, positions)
     rows = positions.shape[0]
     k = positions.new_empty((rows, kv_heads * dim), dtype=torch.bfloat16)
@@ -176,8 +180,10 @@ def cache_rows_4bit(pools, positions: torch.Tensor, row_entry: torch.Tensor, blo
     return k, v
 
 
-def _attention_shape(what: str, q: torch.Tensor, pools, q_heads: int, window: int) -> tuple:
+def _attention_shape(what: str, q: torch.Tensor, pools, block_table: torch.Tensor, q_heads: int, window: int) -> tuple:
     pages, kv_heads, page_tokens, dim = four_bit_dims(pools)
+    if block_table is None or block_table.dim() != 2:
+        raise KernelError(f"{what}: a block table is int32 [entries, blocks]")
     if q.dim() != 2 or q.shape[1] != q_heads * dim or q_heads <= 0 or q_heads % kv_heads:
         raise KernelError(f"{what}: queries {tuple(q.shape)} are not {q_heads} heads of {dim} over {kv_heads} kv heads")
     if window < 0:
@@ -220,10 +226,10 @@ def attention_rows_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_ent
     float.  Each row attends its request's cached keys up to its own position (the last ``window`` of them).  ``max_context`` (0: what
     the block table reaches) only steers into how many parts a row's keys are cut."""
     what = "attention_rows_4bit"
-    kv_heads, page_tokens, dim = _attention_shape(what, q, pools, q_heads, window)
+    kv_heads, page_tokens, dim = _attention_shape(what, q, pools, block_table, q_heads, window)
     rows = q.shape[0]
     if splits is None:
-        keys = max_context or block_table.shape[-1] * page_tokens
+        keys = max_context or block_table.shape[1] * page_tokens
         keys = min(keys, window) if window else keys
         splits = four_bit_row_splits(rows * kv_heads * (-(-(q_heads // kv_heads) // 4)), keys, compute_units(q.device))
     device = _current(what, q)
@@ -257,12 +263,12 @@ def attention_decode_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_e
     """``attention_decode`` over a cache of 4 bits an element: split-KV attention of single rows on the matrix cores, bfloat16
     (``four_bit_decode_supported``).  ``max_context`` (0: what the block table reaches) only steers the number of splits."""
     what = "attention_decode_4bit"
-    kv_heads, page_tokens, dim = _attention_shape(what, q, pools, q_heads, window)
+    kv_heads, page_tokens, dim = _attention_shape(what, q, pools, block_table, q_heads, window)
     if not four_bit_decode_supported(q.dtype, dim, page_tokens):
         raise KernelError(f"{what}: {q.dtype} heads of {dim} in pages of {page_tokens} tokens (attention_rows_4bit takes those)")
     rows, group = q.shape[0], q_heads // kv_heads
     if splits is None:
-        keys = max_context or block_table.shape[-1] * page_tokens
+        keys = max_context or block_table.shape[1] * page_tokens
         splits = four_bit_decode_splits(rows * kv_heads * -(-group // (16 if dim <= 128 else 8)), min(keys, window) if window else keys,
                                         compute_units(q.device))
     device = _current(what, q)
@@ -288,13 +294,11 @@ def attention_prefill_4bit(q: torch.Tensor, out: torch.Tensor, pools, positions:
     covers, into ``out``; other rows of ``out``, and rows from ``covered_rows`` on, are left as they are.  ``tiles``, ``mean_keys`` and
     ``covered_rows`` as there.  A key in sight of a group of tiles whose place has no page makes the group's rows NaN."""
     what = "attention_prefill_4bit"
-    kv_heads, page_tokens, dim = _attention_shape(what, q, pools, q_heads, window)
+    kv_heads, page_tokens, dim = _attention_shape(what, q, pools, block_table, q_heads, window)
     if not four_bit_prefill_supported(q.dtype, dim, page_tokens):
         raise KernelError(f"{what}: {q.dtype} heads of {dim} in pages of {page_tokens} tokens (attention_decode_4bit and attention_rows_4bit take those)")
-    if tiles.dim() != 2 or tiles.shape[1] != 3 or tiles.shape[0] % PREFILL_GROUP_TILES:
+    if tiles is None or tiles.dim() != 2 or tiles.shape[1] != 3 or tiles.shape[0] % PREFILL_GROUP_TILES:
         raise KernelError(f"{what}: tiles must be int32 [n, 3] with n a multiple of {PREFILL_GROUP_TILES}")
-    if block_table.dim() != 2:
-        raise KernelError(f"{what}: a block table is int32 [entries, blocks]")
     rows, groups = q.shape[0], tiles.shape[0] // PREFILL_GROUP_TILES
     if splits is None:
         splits = choose_prefill_splits(groups, q_heads, mean_keys, window, compute_units(q.device))
