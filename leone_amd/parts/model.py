@@ -277,7 +277,8 @@ class DecoderModel:
         """Cache slot -> what the layer runs on it need (one need per slot).  A layer that needs several kinds
         of storage (``cache_need()`` answers with a dict, see ``parts.base.flatten_needs``) gets one slot for
         each, keyed (the run's slot, *names).  ``bits`` 4: keys and values in 4 bits an element (``FourBitKvNeed``), which
-        every layer that caches a token's vectors has to take; state a request keeps stays what it is."""
+        every layer that caches a token's vectors has to take, and one at least has to be there; state a request keeps stays what
+        it is."""
         if bits not in (None, 4):
             raise ValueError(f"a cache of {bits} bits an element is not known; 4, or the model's own type (None)")
         needs: Dict[object, object] = {}
@@ -307,6 +308,8 @@ class DecoderModel:
             if count != 1:
                 raise ValueError(f"cache slot {slot} must have exactly one writing run, found {count}")
         if bits is not None:
+            if not any(getattr(leaf, "four_bits", False) for leaf in needs.values()):
+                raise ValueError("the model caches no keys and values that 4 bits an element could hold")
             needs = {key: leaf.in_four_bits() if getattr(leaf, "four_bits", False) else leaf for key, leaf in needs.items()}
         return needs
 
