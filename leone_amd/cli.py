@@ -91,7 +91,8 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--single-weight-copy", action="store_true",
                    help="Keep no second copy of the matrices in the decode kernels' order (half the weight memory, slower decoding)")
     g.add_argument("--cache-bits", type=int, choices=[4], default=None,
-                   help="Keep keys and values in 4 bits an element: 3.76 times the tokens in the memory of a bfloat16 cache (the model's type)")
+                   help="Keep keys and values in 4 bits an element: 3.76 times the tokens in the memory of a bfloat16 cache, long contexts decode faster; "
+                        "prompts in float32, or with heads of other sizes than 64, 128 and 256, are slower (default: the model's type)")
     g.add_argument("--tune-products", action="store_true",
                    help="Time the vendor library's algorithms for a full prompt portion first and use the fastest (a few seconds)")
     _add_sampling(g)
@@ -110,7 +111,7 @@ def build_parser() -> argparse.ArgumentParser:
     e.add_argument("--position-limit", type=int, default=None, help="Stop after n positions")
     e.add_argument("--prefill-chunk", type=int, default=None, help="Cut every window into portions of n tokens")
     e.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
-    e.add_argument("--cache-bits", type=int, choices=[4], default=None, help="Keep keys and values in 4 bits an element (the model's type)")
+    e.add_argument("--cache-bits", type=int, choices=[4], default=None, help="Keep keys and values in 4 bits an element (default: the model's type)")
 
     r = sub.add_parser("random-model", help="Write a model folder with seeded random weights")
     r.add_argument("--config", required=True, help="config.json to build from")

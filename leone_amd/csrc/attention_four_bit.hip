@@ -15,9 +15,9 @@
 //    smaller ones are off by up to 2^-22 of it.  Heads of 64 hold both parts in one product, the keys given twice.
 //    The instruction adds eight neighbouring elements' products as multiples of 2^-13 of the power of two in the largest of them, cut
 //    towards zero (measured; a product has six bits, so that what lies within 2^8 of the largest is whole), and the eights' sums in
-//    float.  A score is off by at most seven times 2^-13 of its eights' largest products, which seldom shows beside the weights'
-//    rounding: with every eighth element of a query 512 times the others the mean error of a result is 9.6e-4, with float products
-//    8.1e-4 (scores ten wide, results of 0.63).
+//    float.  A score is off by less than 2^-10 of its eights' largest products, which seldom shows beside the weights' rounding: with every
+//    eighth element of a query 512 times the others the mean error of a result is 9.6e-4, with float products 8.1e-4 (scores ten
+//    wide, results of 0.63).
 //  * the values are unpacked by the chip's own conversion, two to an instruction with their power, and brought from neighbouring
 //    elements of a token to neighbouring tokens of an element by one byte permutation for two.  The second product is then
 //    v_mfma_f32_16x16x32_bf16 on exact values; its weights are rounded to bfloat16, against a reference that is a whole number, so
@@ -540,7 +540,9 @@ four_bit_decode_kernel(const bf16_t* __restrict__ q, bf16_t* __restrict__ out, F
 }
 
 // The merge of shares.  kGroup neighbouring lanes have a row and head, four elements each; between them they hold the shares' maxima and
-// sums and hand the weights round, four shares' sums on their way at a time.
+// sums and hand the weights round, four shares' sums on their way at a time.  (A merge of its own beside those of attention_merge.h: they
+// give bfloat16 alone; the one over rows multiplies the sums of every share, also of those that the prompt kernel never wrote, and the
+// one over tiles leaves out what weighs nothing, a NaN with it.)
 constexpr int kMergeThreads = 256;
 constexpr int kMergeAhead = 4;
 constexpr float kNotWritten = -1.f;                              // in a weight's place: a share of no keys, whose sums may be anything

@@ -11,9 +11,9 @@
 // the next, in bfloat16, where v_mfma_f32_32x32x16_bf16 takes them.  Both come by way of registers, asked for two stages ahead: loads
 // that write to shared memory themselves are waited for before it is read again.
 //
-// 2,048 rows behind 8,192 tokens, 32 heads of 128 over 8: 281 us, 1,100 TFLOP/s of the exact work (a product of two 8,192-square bfloat16
-// matrices reaches 1,200 by the vendor library, the bfloat16 prompt kernel 927 here); 128 rows behind 30,720, 64 heads: 131 to 143 us in 8 ranges
-// and their merge, 8 of them.  A pass of 32 keys is 512 cycles of the matrix cores and 560 of vector instructions (a weight is an
+// 2,048 rows behind 8,192 tokens, 32 heads of 128 over 8: 276 to 284 us among other calls, 304 to 312 over and over on the same inputs; at 281
+// 1,100 TFLOP/s of the exact work (a product of two 8,192-square bfloat16 matrices reaches 1,200 by the vendor library, the bfloat16 prompt
+// kernel 933 here); 128 rows behind 30,720, 64 heads: 131 to 143 us in 8 ranges and their merge, 8 of them.  A pass of 32 keys is 512 cycles of the matrix cores and 560 of vector instructions (a weight is an
 // exponential, a value a conversion and a permutation), and the two waves of a SIMD overlap them in part: the matrix cores are busy 45 %
 // of the time, the vector units 47 %.  Forcing the overlap does not pay: two heads a workgroup, four waves a phase behind the other four
 // with a barrier a phase 382 us; a pass's products asked for before the last one's weights 321; two heads a wave 481.

@@ -3,7 +3,8 @@
 // (MXFP4 of the Open Compute Project's Microscaling specification, which this chip's matrix instructions and conversions
 // take as it is).  The power is the smallest whose sevenfold is not below the block's largest magnitude: numbers up to 7
 // round to 6, so that nothing is off by more than one unit, the most that is lost between 4 and 6 as well.  A block with a NaN or an
-// infinity in it gets byte 255 and stands for NaN.
+// infinity in it gets byte 255 and stands for NaN.  (Numbers from 1.75 x 2^127 up round to 2^128 or more, which is an infinity as a
+// bfloat16 or a float.)
 //
 // Layout, P tokens a page:
 //   key codes     [page][kv head][dim / 32][P][16 bytes]          a block: what a lane of the first product takes

@@ -164,7 +164,7 @@ def qk_norm_rope_write_4bit(qkv: torch.Tensor, q_heads: int, kv_heads: int, head
 
 def cache_rows_4bit(pools, positions: torch.Tensor, row_entry: torch.Tensor, block_table: torch.Tensor) -> tuple:
     """The keys and values that a cache of 4 bits an element holds at the rows' positions, bfloat16 ``[rows, kv_heads * dim]`` each (a code
-    times its power is a bfloat16 as it is).  Rows without a page give NaN."""
+    times its power is a bfloat16 as it is, or from 2^128 on an infinity).  Rows without a page give NaN."""
     what = "cache_rows_4bit"
     pages, kv_heads, page_tokens, dim = four_bit_dims(pools)
     if positions is None:
@@ -224,7 +224,8 @@ def attention_rows_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_ent
                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``attention_rows`` over a cache of 4 bits an element: any head size the cache holds, bfloat16 or float32 queries, all arithmetic in
     float.  Each row attends its request's cached keys up to its own position (the last ``window`` of them).  ``max_context`` (0: what
-    the block table reaches) only steers into how many parts a row's keys are cut."""
+    the block table reaches) only steers into how many parts a row's keys are cut.  So does the number of rows: the last bits of a row's
+    result may differ with the rows beside it (a given ``splits`` keeps them)."""
     what = "attention_rows_4bit"
     kv_heads, page_tokens, dim = _attention_shape(what, q, pools, block_table, q_heads, window)
     rows = q.shape[0]
@@ -261,7 +262,8 @@ def attention_decode_4bit(q: torch.Tensor, pools, positions: torch.Tensor, row_e
                           scale: float, window: int = 0, max_context: int = 0, splits: Optional[int] = None,
                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``attention_decode`` over a cache of 4 bits an element: split-KV attention of single rows on the matrix cores, bfloat16
-    (``four_bit_decode_supported``).  ``max_context`` (0: what the block table reaches) only steers the number of splits."""
+    (``four_bit_decode_supported``).  ``max_context`` (0: what the block table reaches) only steers the number of splits.  A score is off by
+    less than 2^-10 of the largest product in each eight neighbouring elements, and weights are rounded to bfloat16."""
     what = "attention_decode_4bit"
     kv_heads, page_tokens, dim = _attention_shape(what, q, pools, block_table, q_heads, window)
     if not four_bit_decode_supported(q.dtype, dim, page_tokens):
@@ -292,7 +294,9 @@ def attention_prefill_4bit(q: torch.Tensor, out: torch.Tensor, pools, positions:
                            covered_rows: Optional[int] = None) -> torch.Tensor:
     """``attention_prefill`` over a cache of 4 bits an element (``four_bit_prefill_supported``): attention for the rows that ``tiles``
     covers, into ``out``; other rows of ``out``, and rows from ``covered_rows`` on, are left as they are.  ``tiles``, ``mean_keys`` and
-    ``covered_rows`` as there.  A key in sight of a group of tiles whose place has no page makes the group's rows NaN."""
+    ``covered_rows`` as there; precision as ``attention_decode_4bit``.  A key in sight of a group of tiles whose place has no page makes the group's rows NaN.
+    The keys are cut into ranges by the bfloat16 kernel's rule (``choose_prefill_splits``), which holds here too: the best of 1 to 32 in nine
+    of twelve shapes of 64 to 2,048 rows behind 0 to 30,720, 2 us off it in two, 8 % in one."""
     what = "attention_prefill_4bit"
     kv_heads, page_tokens, dim = _attention_shape(what, q, pools, block_table, q_heads, window)
     if not four_bit_prefill_supported(q.dtype, dim, page_tokens):
