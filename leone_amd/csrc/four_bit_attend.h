@@ -18,7 +18,7 @@ constexpr float kRaise = 8.0f;                     // a score this far above the
 __device__ inline intx8 low_half(uint4 v) { return intx8{static_cast<int>(v.x), static_cast<int>(v.y), static_cast<int>(v.z), static_cast<int>(v.w), 0, 0, 0, 0}; }
 
 // A query row as two 8-bit parts: sixteen elements a call, `unit` 2^-e with the row's largest element in [2^7, 2^8) units.  The rest is
-// at most half of the first part's last place, sixteen units: times 32 it has the same range.
+// at most half of the first part's last place, which is sixteen units at most: times 32 it is no larger than 2^8.
 __device__ inline void two_parts(const uint4 raw[2], float unit, int high[4], int low[4]) {
     const unsigned w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
 #pragma unroll
@@ -40,7 +40,8 @@ __device__ inline unsigned largest_bits(uint4 v, unsigned top) {          // of 
     for (int i = 0; i < 4; ++i) top = max(max(top, w[i] & 0x7fff0000u), w[i] << 16 & 0x7fff0000u);
     return top;
 }
-// The power byte of a row's first part, from its largest element's bits: 255 where it is no number (its scores are then NaN).
+// The power byte of a row's first part, from its largest element's bits: 255 where it is no number (its scores are then NaN).  It is at
+// least 6, so that the rest's is at least 1: rows of nothing larger than 2^-114 keep fewer bits.
 __device__ inline int query_power(unsigned top) {
     const int exponent = static_cast<int>(top >> 23);
     return exponent == 0xff ? kNanPower : max(exponent - 7, 6);

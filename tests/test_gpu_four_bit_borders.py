@@ -91,3 +91,37 @@ def test_the_largest_numbers():
                 # (what 2^128 is as a float and a bfloat16)
                 assert torch.equal(back[row].double(), torch.where(want[row].abs() >= 2.0 ** 128, want[row] * math.inf, want[row])), row
         assert torch.isfinite(read[0][:2]).all() and torch.isinf(read[0][3:7, 0]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_smallest_numbers(dtype):
+    """Blocks of the least power there is, 2^-126, whose elements are numbers below float's least normal one: kept and read back as they are,
+    and attended as such (a value of which is all that is seen comes out as it is)."""
+    dim, page = 64, 16
+    steps = torch.arange(0, 64, dtype=torch.float64) / 8 * 2.0 ** -126              # 0 to 7 7/8 units in eighths
+    x = torch.stack([steps[:dim], -steps[:dim], steps[:dim] / 4, (steps[:dim] * 2.0 ** -7)]).to(dtype).to(DEVICE)
+    n = x.shape[0]
+    positions = torch.arange(n, dtype=torch.int32, device=DEVICE)
+    entries, table = torch.zeros_like(positions), torch.zeros(1, 1, dtype=torch.int32, device=DEVICE)
+    pools = ops.four_bit_pools(1, 1, dim, page, DEVICE)
+    ops.qk_norm_rope_write_4bit(x.repeat(1, 3).contiguous(), 1, 1, dim, None, None, 1e-6, None, None, positions, entries, table, pools)
+    want = quantised(x).cpu()
+    kept = [p.cpu() for p in pools]
+    read = [r.cpu().double() for r in ops.cache_rows_4bit(pools, positions, entries, table)]
+    for row in range(n):
+        for got, back in zip(held(kept, 0, 0, row), read):
+            assert torch.equal(got, want[row]) and torch.equal(back[row], want[row]), row
+    one = torch.zeros_like(positions)
+    q = torch.zeros(n, dim, dtype=dtype, device=DEVICE)
+    for row in range(n):
+        at = torch.full((1,), row, dtype=torch.int32, device=DEVICE)
+        outs = [ops.attention_rows_4bit(q[:1], pools, at, one[:1], table, 1, 1.0, 1)]
+        if dtype == torch.bfloat16:
+            outs.append(ops.attention_decode_4bit(q[:1], pools, at, one[:1], table, 1, 1.0, 1))
+            tiles = torch.tensor([(0, 0, 1)] + [(0, 0, 0)] * 3, dtype=torch.int32, device=DEVICE)
+            outs.append(ops.attention_prefill_4bit(q[:1], torch.zeros_like(q[:1]), pools, at, tiles, table, 1, 1.0, 1))
+        for out in outs:
+            # (below the least normal number what a product or a sum gives may be nothing)
+            got = out[0].double().cpu()
+            assert torch.equal(torch.where(want[row].abs() >= 2.0 ** -126, got, 0.0), torch.where(want[row].abs() >= 2.0 ** -126, want[row], 0.0)), row
+            assert (got - want[row]).abs().max() < 2.0 ** -126

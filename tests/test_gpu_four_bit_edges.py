@@ -55,3 +55,37 @@ def test_a_value_that_is_no_number_counts_however_little_it_weighs(operator, dim
     assert spoiled.sum() == 2 * 32
     assert torch.equal(torch.isnan(out), spoiled.expand_as(out))
     assert torch.equal(out[:, ~spoiled], before.reshape(rows, q_heads, dim)[:, ~spoiled])
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+def test_portions_recorded_and_replayed(splits):
+    """A portion's attention in a recorded run, its ranges' merge with it: every replay, with other work, calls of its own and synchronizations
+    between, gives the eager call's bits, and so does the eager call every time."""
+    dim, heads, q_heads, page, keys, rows = 128, 2, 4, 64, 512, 200
+    pools, table, _, _ = _low_then_high(dim, heads, page, keys, 300)
+    gen = torch.Generator(device=DEVICE).manual_seed(3)
+    positions = torch.arange(keys - rows, keys, dtype=torch.int32, device=DEVICE)
+    tiles = ops.prefill_tiles([(0, 0, rows)]).to(DEVICE)
+    inputs = [torch.randn(rows, q_heads * dim, generator=gen, device=DEVICE).to(torch.bfloat16) for _ in range(3)]
+    given, out = inputs[0].clone(), torch.zeros_like(inputs[0])
+
+    def call(into):
+        return ops.attention_prefill_4bit(given, into, pools, positions, tiles, table, q_heads, dim ** -0.5, splits=splits)
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        call(out)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            call(out)
+    for turn in range(5):
+        given.copy_(inputs[turn % 3])
+        out.fill_(7.0)
+        stream.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(stream):
+            graph.replay()
+        torch.cuda.synchronize()
+        want = call(torch.zeros_like(out))
+        assert torch.equal(out, want) and torch.equal(want, call(torch.full_like(out, 3.0))), turn
+        torch.randn(1 << 18, generator=gen, device=DEVICE).sum().item()
