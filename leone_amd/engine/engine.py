@@ -215,7 +215,8 @@ class Engine:
                  cache_bits: Optional[int] = None):
         """``cache_bits`` 4: keys and values are kept in 4 bits an element and a power of two for every 32 (``ops.FourBitPools``): 3.76
         times the tokens in the memory of a bfloat16 cache, and as much less to read a step, for coarser keys and values (None: the
-        model's type).  Models of plain attention take it (``DecoderModel.cache_needs``)."""
+        model's type).  Models of plain attention take it (``DecoderModel.cache_needs``).  Prompts in float32, or with heads of other sizes than
+        64, 128 and 256, are slower over it, and a float32 row's last bits may differ with the rows beside it in a step."""
         if model.embedding is None:
             raise ValueError("the model has no weights bound")
         if not torch.cuda.is_available() or model.device.type != "cuda":
